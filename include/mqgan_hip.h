@@ -652,6 +652,83 @@ int mq_comm_init(mqComm **comm, int world, int rank, const void *id_host);
 int mq_allreduce_bucket(mqComm *comm, float *buf, size_t n, mqStream stream);
 int mq_comm_destroy(mqComm *comm);
 
+/* ------------------------------------------------------------------ scores over codes: balance loss, draws
+ * No reference code: the reference's quantiser is FSQ (every code has its cell), its decode (preencoder.py:453-504) takes indices that
+ * somebody else chose.  Scores are (rows, codes) with unit stride along the codes and `row_stride` elements between rows; dtype 0 f32,
+ * 1 bf16, 2 f16; padded: uint8 per row, 1 = padded, or NULL.
+ *
+ * Balance loss: p_n = softmax(z_n), P = mean of p_n over the Nv valid rows, f_e = counts_e / (Nv K) from the K assignments of every
+ * valid row (idx (rows, K) int32, or int64 with idx64 = 1; an index outside [0, codes) is not counted);  L = codes * sum_e f_e P_e;
+ * dL/dz_ne = gout * codes / Nv * p_ne * (f_e - sum_j f_j p_nj), 0 on padded rows.  No valid row: L = 0.
+ *   sums     leaves {sum_n p_ne (codes), counts (codes), Nv} in sums (2 codes + 1 floats; data-parallel ranks add these up), the counts in
+ *            counts (codes + 1 int32, the last one Nv), and per-row statistics (2 floats a row) for bwd
+ *   final    the loss (1 float) and f (codes floats) from the sums
+ *   bwd      dlogits (rows, codes) dense, of the scores' dtype */
+size_t mq_code_balance_workspace(int64_t rows, int codes);
+int mq_code_balance_sums(const void *logits, int dtype, int64_t row_stride, const void *idx, int idx64, int per_row,
+                         const uint8_t *padded, int64_t rows, int codes, void *stats, int32_t *counts, float *sums, void *workspace,
+                         size_t workspace_bytes, mqStream stream);
+int mq_code_balance_final(const float *sums, int codes, int per_row, float *loss, float *fractions, mqStream stream);
+int mq_code_balance_bwd(const void *logits, int dtype, int64_t row_stride, const uint8_t *padded, int64_t rows, int codes,
+                        const void *stats, const float *sums, const float *fractions, const float *gout, void *dlogits, mqStream stream);
+
+/* Drawing a code per row from given uniform numbers in [0, 1).  Codes ordered by (score descending, index ascending), w = exp((z - max) /
+ * temperature): top_k keeps the first k (0: all); top_p every code before which less than top_p of the mass that top_k left lies (the
+ * first always; 1: all); min_p those with w >= min_p.  Drawn: the first in index order at which the running mass of the kept exceeds
+ * uniform * (their mass).  temperature <= 0: the first of the order.  Scores of -inf and NaN are never drawn; a row of nothing else, and a
+ * padded one, gives -1 (logp 0).  Where +inf occurs those codes share the draw evenly.  A uniform number outside [0, 1) is taken as the
+ * nearest end.  The four settings come per row (device, f32 / int32) or, where that is NULL, from the descriptor.
+ * idx (rows) int64; logp (rows) f32 or NULL: log of the drawn code's share of the kept mass. */
+typedef struct {
+    int64_t rows, row_stride;
+    int codes, dtype;
+    double temperature, top_p, min_p;
+    int top_k;
+} mqSampleDesc;
+int mq_sample_codes(const mqSampleDesc *desc_host, const void *logits, const float *uniform, const float *temperature,
+                    const int32_t *top_k, const float *top_p, const float *min_p, const uint8_t *padded, int64_t *idx, float *logp,
+                    mqStream stream);
+
+/* ------------------------------------------------------------------ AdamW over many tensors
+ * Beside mq_adam_step (train.py:312, :401-407): decoupled weight decay, tensors wherever they are, moments in f32 or 8 bits.
+ *   coef = grad_scale * min(1, max_norm / (|grad_scale| * |g|_2 + 1e-6))          the norm over all tensors of the call; max_norm 0: off
+ *   m += (coef g - m)(1 - beta1);  v = beta2 v + (1 - beta2)(coef g)^2
+ *   p = p (1 - lr wd) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)   lr = desc.lr * tensor.lr_scale, t = its own steps
+ * 8-bit moments: groups of 256 elements share a byte `base`; a magnitude is bitcast((c + 8 base) << 20) for its code c > 0, 0 for c = 0; m
+ * has a sign and 7 bits of c (126 infinite, 127 NaN), v 8 bits (254, 255).  Rounded stochastically with a hash of (seed, call, position).
+ *   table_fill   host: checks the tensors and lays out what the step reads, into table_host (table_bytes()); the caller copies it to the
+ *                device.  It holds addresses: fill it again when a tensor moves.
+ *   control      control_bytes(n) device bytes, zeroed by the caller once: the norm's square (f64 at byte 0), the calls so far (int64 at 8),
+ *                and from byte 64 on 16 bytes per tensor whose first int32 is the tensor's step count t
+ *   workspace    device bytes for the norm's partial sums; one step at a time may use control and workspace
+ *   step         grads_host: n device addresses, NULL = no gradient (that tensor, its moments and its step count stay as they are);
+ *                grad_types_host: 0 f32, 1 bf16, 2 f16 each, or NULL for f32.  Both are read before the call returns.  lr is a value of
+ *                the call: a captured step keeps the lr it was captured with, its step counts and random bits move on. */
+typedef struct {
+    float *param;
+    void *exp_avg, *exp_avg_sq;          /* f32, or codes; room for n rounded up to 256, zero behind n */
+    uint8_t *base_avg, *base_avg_sq;     /* 8 bits: one byte per group of 256 */
+    int64_t n;
+    int64_t position;                    /* of its first moment among all tensors' (a multiple of 256): what the random bits hang on */
+    float weight_decay, lr_scale;
+} mqAdamwTensor;
+typedef struct {
+    int n_tensors, state_bits;           /* 32 or 8 */
+    double lr, beta1, beta2, eps, max_norm, grad_scale;
+    uint64_t seed;
+} mqAdamwDesc;
+size_t mq_adamw_table_bytes(const int64_t *numel_host, int n);
+size_t mq_adamw_control_bytes(int n);
+size_t mq_adamw_workspace(const int64_t *numel_host, int n);
+int mq_adamw_table_fill(const mqAdamwTensor *tensors_host, int n, int state_bits, void *table_host, size_t table_bytes);
+int mq_adamw_step(const mqAdamwDesc *desc_host, const int64_t *numel_host, const void *table, const void *const *grads_host,
+                  const uint8_t *grad_types_host, void *control, void *workspace, size_t workspace_bytes, mqStream stream);
+/* f32 moments to codes (to nearest) and back (f32, or bf16: exact in both), n a multiple of 256 */
+int mq_moments8_encode(const float *exp_avg, const float *exp_avg_sq, int64_t n, uint8_t *codes_avg, uint8_t *base_avg,
+                       uint8_t *codes_avg_sq, uint8_t *base_avg_sq, mqStream stream);
+int mq_moments8_decode(const uint8_t *codes_avg, const uint8_t *base_avg, const uint8_t *codes_avg_sq, const uint8_t *base_avg_sq,
+                       int64_t n, int bf16, void *exp_avg, void *exp_avg_sq, mqStream stream);
+
 /* DEBUG / MEASUREMENT ONLY - the one piece of process-global state in this ABI (everything else is per call and per stream):
  * two function pointers, not thread-safe, meant for ONE measuring thread (bench.py, tools/layer_profile.py) and NULL otherwise;
  * a production caller never sets them, and with both NULL the library keeps no state between calls.

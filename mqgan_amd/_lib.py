@@ -57,6 +57,22 @@ class PointwiseDesc(C.Structure):
                 ("d1", C.c_int64), ("d2", C.c_int64), ("d3", C.c_int64), ("p_drop", C.c_float), ("seed", C.c_uint64)]
 
 
+class SampleDesc(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("row_stride", C.c_int64), ("codes", C.c_int), ("dtype", C.c_int), ("temperature", C.c_double),
+                ("top_p", C.c_double), ("min_p", C.c_double), ("top_k", C.c_int)]
+
+
+class AdamwTensor(C.Structure):
+    _fields_ = [("param", C.c_void_p), ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("base_avg", C.c_void_p),
+                ("base_avg_sq", C.c_void_p), ("n", C.c_int64), ("position", C.c_int64), ("weight_decay", C.c_float),
+                ("lr_scale", C.c_float)]
+
+
+class AdamwDesc(C.Structure):
+    _fields_ = [("n_tensors", C.c_int), ("state_bits", C.c_int), ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double),
+                ("eps", C.c_double), ("max_norm", C.c_double), ("grad_scale", C.c_double), ("seed", C.c_uint64)]
+
+
 _P, _I, _L, _F, _D, _Z, _U64 = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_double, C.c_size_t, C.c_uint64
 
 # name -> (restype, argtypes); every symbol declared in include/mqgan_hip.h
@@ -174,6 +190,18 @@ SIGNATURES = {
     "mq_multi_gather": (_I, [_P, _I, _L, _P, _P]),
     "mq_multi_gather_args": (_I, [_P, _I, _P, _P]),
     "mq_adam_step": (_I, [_P, _P, _P, _P, _L, _D, _D, _D, _D, _I, _P, _F, _F, _P]),
+    "mq_code_balance_workspace": (_Z, [_L, _I]),
+    "mq_code_balance_sums": (_I, [_P, _I, _L, _P, _I, _I, _P, _L, _I, _P, _P, _P, _P, _Z, _P]),
+    "mq_code_balance_final": (_I, [_P, _I, _I, _P, _P, _P]),
+    "mq_code_balance_bwd": (_I, [_P, _I, _L, _P, _L, _I, _P, _P, _P, _P, _P, _P]),
+    "mq_sample_codes": (_I, [C.POINTER(SampleDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "mq_adamw_table_bytes": (_Z, [_P, _I]),
+    "mq_adamw_control_bytes": (_Z, [_I]),
+    "mq_adamw_workspace": (_Z, [_P, _I]),
+    "mq_adamw_table_fill": (_I, [C.POINTER(AdamwTensor), _I, _I, _P, _Z]),
+    "mq_adamw_step": (_I, [C.POINTER(AdamwDesc), _P, _P, _P, _P, _P, _P, _Z, _P]),
+    "mq_moments8_encode": (_I, [_P, _P, _L, _P, _P, _P, _P, _P]),
+    "mq_moments8_decode": (_I, [_P, _P, _P, _P, _L, _I, _P, _P, _P]),
     "mq_comm_unique_id": (_I, [_P]),
     "mq_comm_init": (_I, [C.POINTER(_P), _I, _I, _P]),
     "mq_allreduce_bucket": (_I, [_P, _P, _Z, _P]),

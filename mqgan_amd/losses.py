@@ -154,3 +154,15 @@ def masked_mae(pred, target, mask, eps: float = 1e-8, comm: Comm = None, leaky_s
     """train.py:38-45 on channels-last features (B, H, W, C) with a uint8 padded mask (B, W).  ``leaky_slope``: pred is a
     feature map of a discriminator run with ``pregate=True`` (the LeakyReLU backward of its layer rides on this gradient)."""
     return ops.MaskedMaeFn.apply(ops.to_f32(pred).contiguous(), ops.to_f32(target).contiguous(), mask, comm, leaky_slope)
+
+
+def code_balance_loss(logits, idx, padded=None, comm: Comm = None):
+    """Balance loss of a codebook and how often each code was used: logits (..., E) f32 / bf16 / f16 scores, ``idx`` (...) or (..., K) int32 /
+    int64 assignments, ``padded`` (...) uint8 / bool, 1 = padded -> (loss f32 scalar, counts (E,) int32).
+
+        loss = E sum_e f_e P_e,   P_e = mean over the valid rows of softmax(logits)_e,   f_e = counts_e / (valid rows K)
+
+    1 where the codes are used evenly, up to E where one takes all.  The gradient goes to the scores (through P; counts are whole numbers);
+    it is 0 on padded rows, whose scores are not read.  An index outside [0, E) is not counted.  No valid row: loss 0.  With ``comm`` sums and
+    counts are those of all ranks (exact up to 2^24 a code), and the ranks' gradients add up to the whole batch's."""
+    return ops.CodeBalanceFn.apply(logits, idx, padded, comm)

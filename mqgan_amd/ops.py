@@ -1589,6 +1589,128 @@ def codebook_ema_update(x, idx, cluster_size, embed_sum, codebook, decay=0.99, e
                                      fptr(codebook), ptr(ws), nbytes, stream()), "mq_codebook_ema_update")
 
 
+# ----------------------------------------------------------------------------- scores over codes
+_SCORE_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _score_rows(logits: torch.Tensor, what: str):
+    """(scores, their type's number, rows, codes, elements between rows): unit stride along the codes and one stride between all rows is
+    read in place (a slice of a wider head's output), anything else is copied."""
+    kind = _SCORE_TYPES.get(logits.dtype)
+    if kind is None or logits.dim() < 1:
+        raise _lib.MqganHipError(f"{what}: scores are f32, bf16 or f16 with the codes in the last dimension, got {logits.dtype} {tuple(logits.shape)}")
+    V = logits.shape[-1]
+    if V == 0:
+        raise _lib.MqganHipError(f"{what}: no codes")
+    rows = logits.numel() // V
+    z = logits.detach()
+    stride, ok = V, z.stride(-1) == 1 or V == 1
+    dims = [(n, s) for n, s in zip(z.shape[:-1], z.stride()[:-1]) if n != 1]
+    if dims:
+        stride = dims[-1][1]
+        ok = ok and stride >= V and all(a[1] == b[0] * b[1] for a, b in zip(dims, dims[1:]))
+    if not ok:
+        z, stride = z.contiguous(), V
+    return z, kind, rows, V, stride
+
+
+def _score_ptr(z):
+    """Device pointer of scores that _score_rows has checked (rows may lie apart)."""
+    if not z.is_cuda or z.device.index != torch.cuda.current_device():
+        ptr(z)                                      # raises with the reason
+        raise _lib.MqganHipError(f"tensor lives on {z.device}")
+    return C.c_void_p(z.data_ptr())
+
+
+def _row_mask(padded, rows, like, what):
+    if padded is None:
+        return None
+    if padded.dtype not in (torch.uint8, torch.bool) or padded.numel() != rows:
+        raise _lib.MqganHipError(f"{what}: padded is uint8 or bool with one value per row ({rows}), got {padded.dtype} {tuple(padded.shape)}")
+    return padded.reshape(-1).to(torch.uint8).contiguous()
+
+
+def sample_codes(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, padded=None, return_logp=False):
+    """Draw a code per row: logits (..., V) f32 / bf16 / f16, ``uniform`` (...) f32 in [0, 1) -> int64 codes (...) [, f32 log of the drawn
+    code's share of what was kept].  The codes in order of (score descending, index ascending), w = exp((z - max) / temperature): ``top_k``
+    keeps the first k (0: all), ``top_p`` every code before which less than top_p of their mass lies (1: all), ``min_p`` those with
+    w >= min_p; drawn is the first code, in index order, at which the running mass exceeds uniform times the mass of all kept ones.
+    temperature 0: the largest score, lowest index.  Each setting is a number or a tensor with one value per row.  Scores of -inf and NaN
+    are never drawn; a row of nothing else, and a ``padded`` one (uint8 / bool, 1 = padded), gives -1.  Masses are exact whole numbers
+    (csrc/sample.hip): the same inputs draw the same codes on every run."""
+    z, kind, rows, V, stride = _score_rows(logits, "sample_codes")
+    shape = logits.shape[:-1]
+    if uniform.dtype != F32 or uniform.numel() != rows:
+        raise _lib.MqganHipError(f"sample_codes: one f32 uniform number per row ({rows}), got {uniform.dtype} {tuple(uniform.shape)}")
+    idx = torch.empty(shape, dtype=torch.int64, device=z.device)
+    logp = _empty(shape, z) if return_logp else None
+    if rows:
+        held = {}
+
+        def setting(name, v, dtype):
+            if not isinstance(v, torch.Tensor):
+                return None
+            if v.numel() != rows:
+                raise _lib.MqganHipError(f"sample_codes: {name} is a number or has one value per row ({rows}), got {tuple(v.shape)}")
+            held[name] = v.reshape(-1).to(dtype).contiguous()
+            return held[name]
+        t, k = setting("temperature", temperature, F32), setting("top_k", top_k, torch.int32)
+        p, m = setting("top_p", top_p, F32), setting("min_p", min_p, F32)
+        mask, u = _row_mask(padded, rows, z, "sample_codes"), uniform.reshape(-1).contiguous()
+        d = _lib.SampleDesc(rows, stride, V, kind, 0.0 if t is not None else float(temperature), 0.0 if p is not None else float(top_p),
+                            0.0 if m is not None else float(min_p), 0 if k is not None else min(int(top_k), V))
+        check(L().mq_sample_codes(C.byref(d), _score_ptr(z), fptr(u), fptr(t, True), ptr(k, torch.int32, True), fptr(p, True), fptr(m, True),
+                                  ptr(mask, torch.uint8, True), ptr(idx, torch.int64), fptr(logp, True), stream()), "mq_sample_codes")
+    return (idx, logp) if return_logp else idx
+
+
+class CodeBalanceFn(torch.autograd.Function):
+    """(loss, counts) of losses.code_balance_loss."""
+
+    @staticmethod
+    def forward(ctx, logits, idx, padded, comm):
+        z, kind, rows, V, stride = _score_rows(logits, "code_balance_loss")
+        K = idx.shape[-1] if idx.dim() == logits.dim() else 1
+        if idx.dtype not in (torch.int32, torch.int64) or tuple(idx.shape) not in (tuple(logits.shape[:-1]), tuple(logits.shape[:-1]) + (K,)):
+            raise _lib.MqganHipError(f"code_balance_loss: int32 / int64 codes of shape {tuple(logits.shape[:-1])} or with the assignments of a row "
+                                     f"behind, got {idx.dtype} {tuple(idx.shape)}")
+        mask = _row_mask(padded, rows, z, "code_balance_loss")
+        sums = _empty((2 * V + 1,), z)
+        counts = torch.empty((V + 1,), dtype=torch.int32, device=z.device)
+        stats = _empty((max(rows, 1), 2), z)
+        idx = idx.contiguous()
+        if rows and K:
+            nbytes = L().mq_code_balance_workspace(rows, V)
+            ws = _ws_bytes(nbytes, z)
+            check(L().mq_code_balance_sums(_score_ptr(z), kind, stride, ptr(idx), int(idx.dtype == torch.int64), K, ptr(mask, torch.uint8, True),
+                                           rows, V, ptr(stats), ptr(counts), fptr(sums), ptr(ws), ws.numel(), stream()), "mq_code_balance_sums")
+        else:
+            sums.zero_()
+            counts.zero_()
+        if comm is not None and comm.active:
+            _reduce(comm, sums)
+            counts = sums[V:].to(torch.int32)
+        loss, f = _empty((1,), z), _empty((V,), z)
+        check(L().mq_code_balance_final(fptr(sums), V, max(K, 1), fptr(loss), fptr(f), stream()), "mq_code_balance_final")
+        ctx.save_for_backward(z, mask, stats, sums, f)
+        ctx.cfg = (kind, rows, V, stride, logits.shape)
+        counts = counts[:V]
+        ctx.mark_non_differentiable(counts)
+        return loss.view(()), counts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gout, _):
+        z, mask, stats, sums, f = ctx.saved_tensors
+        kind, rows, V, stride, shape = ctx.cfg
+        dz = torch.empty(shape, dtype=z.dtype, device=z.device)
+        if rows:
+            g = gout.to(F32).contiguous().view(1)
+            check(L().mq_code_balance_bwd(_score_ptr(z), kind, stride, ptr(mask, torch.uint8, True), rows, V, ptr(stats), fptr(sums), fptr(f),
+                                          fptr(g), ptr(dz), stream()), "mq_code_balance_bwd")
+        return dz, None, None, None
+
+
 # ----------------------------------------------------------------------------- losses
 # Every loss is computed in two halves so that the normalisers can be made global under data parallelism: the *_sums
 # kernels leave numerators and counts in a small device buffer, ``comm.all_reduce_sum`` (identity for one process) sums it

@@ -1,0 +1,247 @@
+"""AdamW over many tensors on the HIP kernels (csrc/adamw.hip): decoupled weight decay, gradient-norm clipping, moments in f32 or
+in 8 bits.  Beside train.FlatAdam, which is torch.optim.Adam (no decay) over one arena; the reference has Adam only (train.py:312).
+
+A step is two or three launches whatever the number of tensors: the squares of the norm (with ``max_norm``), one small block that forms
+the factors, the update.  Everything that changes from step to step is on the device, so a step may be captured into a graph: the replay
+counts on, with the lr and the gradients' addresses of its capture.  One step at a time: a captured step and an eager one of the same
+optimiser run one after the other (they share its workspace).
+"""
+import ctypes as C
+
+import numpy as np
+import torch
+
+from . import _lib
+from ._lib import AdamwDesc, AdamwTensor, MqganHipError, check, ptr, stream
+from .ddp import FlatArena
+
+GROUP = 256                                # elements that share an exponent base; every tensor's moments start on such a boundary
+_GRAD_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_CONTROL = 64                              # bytes of the control buffer in front of the per-tensor states
+
+
+class AdamW:
+    """``params``: a ddp.FlatArena, f32 tensors, or dicts {"params": tensors, "weight_decay": w, "lr_scale": s} (both optional).
+    ``state_bits``: 32, or 8 (two bytes a parameter plus two for every 256; see csrc/adamw.hip for the format).
+    ``decays``: which tensors of an arena decay (a function of the parameter; default all).
+    ``seed``: of the 8-bit moments' random rounding.  A tensor without a gradient is left out of a step, as in torch.optim.AdamW:
+    its moments and its step count stay."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, seed=0, decays=None):
+        self.arena = params if isinstance(params, FlatArena) else None
+        groups = [{"params": params.params}] if self.arena is not None else list(params)
+        if groups and not isinstance(groups[0], dict):
+            groups = [{"params": groups}]
+        self.params, self.weight_decays, self.lr_scales = [], [], []
+        for g in groups:
+            unknown = set(g) - {"params", "weight_decay", "lr_scale"}
+            if unknown:
+                raise ValueError(f"AdamW: a group has params, weight_decay and lr_scale, not {sorted(unknown)}")
+            for p in g["params"]:
+                self.params.append(p)
+                self.weight_decays.append(float(g.get("weight_decay", weight_decay)) if decays is None or decays(p) else 0.0)
+                self.lr_scales.append(float(g.get("lr_scale", 1.0)))
+        if not self.params:
+            raise ValueError("AdamW: no parameters")
+        if len({id(p) for p in self.params}) != len(self.params):
+            raise ValueError("AdamW: a parameter is given twice")
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: moments are held in 8 or 32 bits, not {state_bits}")
+        if not (lr >= 0 and eps >= 0 and all(0 <= b < 1 for b in betas) and len(betas) == 2 and all(w >= 0 for w in self.weight_decays)):
+            raise ValueError("AdamW: lr, eps and weight_decay >= 0 and two betas in [0, 1) are needed")
+        self.device = self.params[0].device
+        for i, p in enumerate(self.params):
+            if not p.is_cuda or p.device != self.device:
+                raise MqganHipError(f"AdamW: parameter {i} lives on {p.device}; every parameter belongs on one HIP device")
+            if p.dtype != torch.float32 or not p.is_contiguous():
+                raise MqganHipError(f"AdamW: parameter {i} is {p.dtype}{'' if p.is_contiguous() else ', not contiguous'}: parameters are "
+                                    "contiguous f32 (they are their own master copy)")
+        self.base_lr = self.lr = float(lr)
+        self.betas, self.eps, self.state_bits, self.seed = (float(betas[0]), float(betas[1])), float(eps), state_bits, int(seed)
+        n = len(self.params)
+        sizes = [p.numel() for p in self.params]
+        self.positions = np.concatenate([[0], np.cumsum([(s + GROUP - 1) // GROUP * GROUP for s in sizes])]).tolist()
+        total = max(self.positions[-1], GROUP)
+        new = lambda k, dt: torch.zeros(k, dtype=dt, device=self.device)  # noqa: E731
+        if state_bits == 32:
+            self.exp_avg, self.exp_avg_sq = new(total, torch.float32), new(total, torch.float32)
+            self._bases = None
+        else:
+            self.exp_avg, self.exp_avg_sq = new(total, torch.uint8), new(total, torch.uint8)
+            self._bases = new(total // GROUP, torch.uint8), new(total // GROUP, torch.uint8)
+        lib = _lib.load()
+        self._sizes = (C.c_int64 * n)(*sizes)
+        self._table_bytes = lib.mq_adamw_table_bytes(self._sizes, n)
+        if not self._table_bytes:
+            raise MqganHipError("AdamW: too many elements")
+        self._control = new(lib.mq_adamw_control_bytes(n) // 8, torch.int64)
+        self._workspace = new(lib.mq_adamw_workspace(self._sizes, n) // 8, torch.float64)
+        self._desc = AdamwDesc(n_tensors=n, state_bits=state_bits, beta1=self.betas[0], beta2=self.betas[1], eps=self.eps, seed=self.seed & (2 ** 64 - 1))
+        self._addresses, self._captured = None, []
+        self._scale = 1.0
+        self._bind([p.data_ptr() for p in self.params])
+
+    # -- tables ---------------------------------------------------------------------------------
+    def _bind(self, addresses):
+        """(Re)build the device table of the tensors' addresses."""
+        if torch.cuda.is_current_stream_capturing():
+            raise MqganHipError("AdamW: a parameter moved since the last step; take one step outside the capture first")
+        n, item = len(self.params), self.exp_avg.element_size()
+        m, v = self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr()
+        mb, vb = (b.data_ptr() for b in self._bases) if self._bases else (0, 0)
+        rows = (AdamwTensor * n)()
+        for i, (a, at) in enumerate(zip(addresses, self.positions)):
+            rows[i] = AdamwTensor(a, m + at * item, v + at * item, mb and mb + at // GROUP, vb and vb + at // GROUP, self._sizes[i], at,
+                                  self.weight_decays[i], self.lr_scales[i])
+        host = torch.empty(self._table_bytes, dtype=torch.uint8)
+        check(_lib.load().mq_adamw_table_fill(rows, n, self.state_bits, C.c_void_p(host.data_ptr()), self._table_bytes), "mq_adamw_table_fill")
+        self._table = host.to(self.device)          # from pageable memory: complete when the call returns
+        self._addresses = addresses
+
+    # -- the step -------------------------------------------------------------------------------
+    def zero_grad(self):
+        if self.arena is not None:
+            self.arena.zero_grad()
+        else:
+            for p in self.params:
+                p.grad = None
+
+    def _gradients(self, grads):
+        if grads is not None:
+            return grads
+        if self.arena is not None and self.arena.gather_mode:
+            self.arena.gather()                     # whatever the reducer has not moved yet; a parameter without gradient is left out
+            flat = self.arena.flat_grad
+            return [None if p.grad is None else flat[o:o + p.numel()] for p, o in zip(self.params, self.arena.offsets)]
+        return [p.grad for p in self.params]
+
+    def step(self, max_norm=0.0, grad_scale=1.0, grads=None):
+        """``max_norm`` > 0: clip the norm of all gradients to it (``grad_norm()`` then has the norm).  ``grad_scale``: factor on every
+        gradient (1 / world size for summed ones).  ``grads``: the gradients (f32, bf16 or f16; None = none) in the order of the
+        parameters, instead of their ``.grad``."""
+        if torch.cuda.current_device() != self.device.index:
+            raise MqganHipError(f"AdamW: the parameters live on {self.device} but the current HIP device is cuda:{torch.cuda.current_device()}")
+        if not max_norm >= 0.0:
+            raise ValueError(f"AdamW: max_norm {max_norm}")
+        params = self.params
+        grads = self._gradients(grads)
+        if len(grads) != len(params):
+            raise MqganHipError(f"AdamW: {len(grads)} gradients for {len(params)} parameters")
+        held, addresses, types = [], [], bytearray(len(params))
+        for i, (g, size) in enumerate(zip(grads, self._sizes)):
+            if g is None:
+                addresses.append(0)
+                continue
+            t = _GRAD_TYPES.get(g.dtype)
+            if t is None or g.numel() != size or g.device != self.device:
+                raise MqganHipError(f"AdamW: gradient {i} is {g.dtype} {tuple(g.shape)} on {g.device}; its parameter is {tuple(params[i].shape)} "
+                                    f"on {self.device}")
+            if not g.is_contiguous():
+                g = g.contiguous()
+                held.append(g)                      # until the launches are enqueued: the stream's order keeps its memory after that
+            types[i] = t
+            addresses.append(g.data_ptr())
+        at = [p.data_ptr() for p in params]
+        if at != self._addresses:
+            for i, p in enumerate(params):
+                if p.dtype != torch.float32 or not p.is_contiguous() or p.numel() != self._sizes[i] or p.device != self.device:
+                    raise MqganHipError(f"AdamW: parameter {i} became {p.dtype} {tuple(p.shape)} on {p.device}")
+            self._bind(at)
+        if torch.cuda.is_current_stream_capturing() and self._table is not (self._captured[-1] if self._captured else None):
+            self._captured.append(self._table)      # a graph reads it as long as it is replayed
+        d = self._desc
+        d.lr, d.max_norm, d.grad_scale = float(self.lr), float(max_norm), float(grad_scale)
+        check(_lib.load().mq_adamw_step(C.byref(d), self._sizes, ptr(self._table), (C.c_void_p * len(params))(*addresses),
+                                        (C.c_uint8 * len(params)).from_buffer(types), ptr(self._control), ptr(self._workspace),
+                                        self._workspace.numel() * 8, stream()), "mq_adamw_step")
+        self._scale = float(grad_scale)
+
+    def grad_norm(self):
+        """Norm of the scaled gradients before clipping, of the last step with ``max_norm`` > 0 (device scalar; reading it synchronises)."""
+        return self._control[:1].view(torch.float64).sqrt()[0].float() * abs(self._scale)
+
+    # -- moments and state ------------------------------------------------------------------------
+    def moments(self, dtype=torch.float32):
+        """(first, second) moments as flat tensors, tensor i's from ``positions[i]`` on, zeros between.  With f32 moments asked for in f32 they
+        are the optimiser's own buffers; 8-bit moments are decoded (exactly, into f32 or bf16)."""
+        if self.state_bits == 32:
+            return self.exp_avg.to(dtype), self.exp_avg_sq.to(dtype)
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise MqganHipError(f"AdamW: 8-bit moments decode into float32 or bfloat16, not {dtype}")
+        m, v = (torch.empty(self.exp_avg.numel(), dtype=dtype, device=self.device) for _ in range(2))
+        check(_lib.load().mq_moments8_decode(ptr(self.exp_avg), ptr(self._bases[0]), ptr(self.exp_avg_sq), ptr(self._bases[1]), m.numel(),
+                                             int(dtype == torch.bfloat16), ptr(m), ptr(v), stream()), "mq_moments8_decode")
+        return m, v
+
+    def load_moments(self, exp_avg, exp_avg_sq, step=None):
+        """Set the moments from flat f32 tensors laid out as ``moments()`` gives them (8 bits: rounded to nearest), and, with ``step``, every
+        tensor's step count and the count of calls."""
+        for x in (exp_avg, exp_avg_sq):
+            if x.numel() != self.exp_avg.numel():
+                raise MqganHipError(f"AdamW: moments of {x.numel()} elements, the layout has {self.exp_avg.numel()}")
+        if self.state_bits == 32:
+            self.exp_avg.copy_(exp_avg.reshape(-1))
+            self.exp_avg_sq.copy_(exp_avg_sq.reshape(-1))
+        else:
+            m, v = (x.to(self.device, torch.float32).reshape(-1).contiguous() for x in (exp_avg, exp_avg_sq))
+            check(_lib.load().mq_moments8_encode(ptr(m), ptr(v), m.numel(), ptr(self.exp_avg), ptr(self._bases[0]), ptr(self.exp_avg_sq),
+                                                 ptr(self._bases[1]), stream()), "mq_moments8_encode")
+        if step is not None:
+            self._set_steps([int(step)] * len(self.params), int(step))
+
+    def _steps(self):
+        """Every tensor's step count, and the calls so far (synchronises)."""
+        host = self._control.cpu()
+        return host[_CONTROL // 8:].view(torch.int32)[::4].tolist(), int(host[1])
+
+    def _set_steps(self, steps, calls):
+        host = self._control.cpu()
+        host[_CONTROL // 8:].view(torch.int32)[::4] = torch.tensor(steps, dtype=torch.int32)
+        host[1] = calls
+        self._control.copy_(host)
+
+    @property
+    def step_count(self):
+        """Steps of the tensor that took most (synchronises)."""
+        return max(self._steps()[0])
+
+    def state_dict(self):
+        """torch.optim.AdamW's format (moments in f32), so a state moves between the two and between 8 and 32 bits; for 8 bits the codes
+        besides, from which a run goes on bit for bit."""
+        steps, calls = self._steps()
+        m, v = self.moments()
+        state = {}
+        for i, (p, at, t) in enumerate(zip(self.params, self.positions, steps)):
+            if t:
+                state[i] = {"step": torch.tensor(float(t)), "exp_avg": m[at:at + p.numel()].view_as(p).clone(),
+                            "exp_avg_sq": v[at:at + p.numel()].view_as(p).clone()}
+        group = {"lr": self.lr, "betas": self.betas, "eps": self.eps, "weight_decay": max(self.weight_decays), "amsgrad": False,
+                 "maximize": False, "foreach": None, "capturable": False, "differentiable": False, "fused": None,
+                 "initial_lr": self.base_lr, "params": list(range(len(self.params)))}
+        sd = {"state": state, "param_groups": [group], "mqgan_amd_calls": calls}
+        if self.state_bits == 8:
+            sd["mqgan_amd_moments8"] = {"codes": (self.exp_avg.clone(), self.exp_avg_sq.clone()), "bases": tuple(b.clone() for b in self._bases),
+                                        "sizes": list(self._sizes)}
+        return sd
+
+    def load_state_dict(self, sd):
+        steps = [0] * len(self.params)
+        total = self.exp_avg.numel()
+        m, v = (torch.zeros(total, dtype=torch.float32, device=self.device) for _ in range(2))
+        for i, st in sd.get("state", {}).items():
+            i = int(i)
+            if i >= len(self.params) or st["exp_avg"].numel() != self._sizes[i]:
+                raise MqganHipError(f"AdamW: the state's entry {i} does not fit the parameters")
+            at = self.positions[i]
+            m[at:at + self._sizes[i]].copy_(st["exp_avg"].reshape(-1))
+            v[at:at + self._sizes[i]].copy_(st["exp_avg_sq"].reshape(-1))
+            steps[i] = int(float(st["step"]))
+        held = sd.get("mqgan_amd_moments8")
+        if self.state_bits == 8 and held is not None and list(held["sizes"]) == list(self._sizes):
+            for mine, theirs in zip((self.exp_avg, self.exp_avg_sq) + self._bases, tuple(held["codes"]) + tuple(held["bases"])):
+                mine.copy_(theirs)
+        else:
+            self.load_moments(m, v)
+        self._set_steps(steps, int(sd.get("mqgan_amd_calls", max(steps))))
+        if sd.get("param_groups"):
+            self.lr = sd["param_groups"][0].get("lr", self.lr)

@@ -238,6 +238,16 @@ class PreEncoder(nn.Module):
         _, indices = self.quantizer(self._encode_latent(x, mask))
         return indices.long()
 
+    @torch.no_grad()
+    def sample(self, logits, uniform, x_mask=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """Indices for ``decode`` out of a token model's scores: logits (B, T, V >= codebook_size; what lies behind the codes - the bos / eos
+        scores among it - takes no part), uniform (B, T) f32 in [0, 1), x_mask bool (B, 1, T) True = padded or None -> int64
+        (B, T), 0 on padded frames.  The settings are ops.sample_codes's.  A frame without a finite score gets 0 as well."""
+        if logits.dim() != 3 or logits.shape[-1] < self.codebook_size:
+            raise ValueError(f"sample: logits (B, T, >= {self.codebook_size}) are needed, got {tuple(logits.shape)}")
+        padded = None if x_mask is None else x_mask.reshape(logits.shape[:2])
+        return ops.sample_codes(logits[..., :self.codebook_size], uniform, temperature, top_k, top_p, min_p, padded).clamp_(min=0)
+
     def decode(self, indices, x_mask=None, return_hidden=False):
         """indices (B, T) -> x_post (B, T, mel) [, last_hid (B, C0, T)].  :453-504."""
         B, T = indices.shape

@@ -171,6 +171,31 @@ class L2Quantizer(nn.Module):
         codes = torch.nn.functional.embedding(idx.long(), self.codebook)      # gather (data movement only)
         return x + (codes - x).detach(), idx
 
+    def scores(self, x: torch.Tensor, temperature: float = 1.0) -> torch.Tensor:
+        """-|x - c|^2 / temperature for every code, up to a term of the vector alone: (..., d) -> (..., codebook_size) f32.  The gradient
+        goes to x (the codebook moves by its EMA)."""
+        if not temperature > 0:
+            raise ValueError(f"L2Quantizer.scores: temperature {temperature}")
+        with torch.no_grad():
+            w, wt = ops.weight_prep(ops.scale(self.codebook, 2.0 / temperature), None, need_crsk=x.requires_grad)
+            bias = ops.scale(ops.l2_codebook_norms(self.codebook), -1.0 / temperature)
+        rows = x.numel() // self.dim
+        d = ops.conv_desc(1, 1, rows, self.dim, self.codebook_size, 1, 1)
+        y = ops.conv(x.reshape(1, 1, rows, self.dim).contiguous(), w, wt, bias, d, out_f32=True)
+        return ops.to_f32(y).view(*x.shape[:-1], self.codebook_size)
+
+    def balance_loss(self, x: torch.Tensor, idx: torch.Tensor, padded=None, temperature: float = 1.0, comm=None):
+        """(loss, counts): losses.code_balance_loss of these vectors' soft assignment and the codes they were given.  Added to a training loss
+        it pulls the vectors towards codes that are used less."""
+        from .losses import code_balance_loss
+        return code_balance_loss(self.scores(x, temperature), idx, padded, comm)
+
+    @torch.no_grad()
+    def draw(self, x: torch.Tensor, uniform: torch.Tensor, temperature: float = 1.0, top_k: int = 0, padded=None) -> torch.Tensor:
+        """A code per vector drawn with probability softmax(-|x - c|^2 / temperature), among the ``top_k`` nearest where that is not 0, from given
+        uniform numbers (...) - instead of the nearest.  int32, as ``indices``; -1 on padded rows."""
+        return ops.sample_codes(self.scores(x, temperature), uniform, top_k=top_k, padded=padded).to(torch.int32)
+
     @torch.no_grad()
     def ema_update(self, x: torch.Tensor, idx: torch.Tensor):
         ops.codebook_ema_update(x.reshape(-1, self.dim).contiguous(), idx.reshape(-1).to(torch.int32).contiguous(),

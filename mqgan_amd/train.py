@@ -30,6 +30,7 @@ from .ddp import FlatArena, GradReducer, broadcast_arena
 from .discriminators import MelSpectrogramPatchDiscriminator2D, MultiBinDiscriminator, run_discriminators
 from .losses import LSGANLoss, masked_mae_deferred, recon_loss_deferred
 from .nn_base import share_effective_weights
+from .optim import AdamW
 from .preencoder import PreEncoder
 
 
@@ -153,7 +154,7 @@ class FlatAdam:
 class WarmupLR:
     """LambdaLR(lr_lambda = min((step + 1) / warmup, 1)) on the generator optimiser (train.py:326-329)."""
 
-    def __init__(self, opt: FlatAdam, warmup_steps: int):
+    def __init__(self, opt, warmup_steps: int):
         self.opt, self.warmup, self.last_epoch = opt, warmup_steps, 0
         opt.lr = opt.base_lr * min(1.0 / warmup_steps, 1.0)
 
@@ -268,7 +269,17 @@ class Trainer:
         return gen, d1, d2
 
     def _init_optimizers(self):
+        """training.optimizer (new key): adam (default, the reference's: train.py:312), adamw or adamw8bit (decoupled training.weight_decay,
+        default 0.01, on tensors with more than one value per output channel; moments in f32 or in 8 bits)."""
         t = self.config["training"]
+        kind = str(t.get("optimizer", "adam")).lower()
+        if kind not in ("adam", "adamw", "adamw8bit"):
+            raise ValueError(f"training.optimizer must be adam, adamw or adamw8bit, got {kind!r}")
+        if kind != "adam":
+            make = partial(AdamW, weight_decay=float(t.get("weight_decay", 0.01)), state_bits=8 if kind == "adamw8bit" else 32, seed=t["seed"],
+                           decays=lambda p: p.dim() > 1 and p.numel() > p.shape[0])
+            return (make(self.arena_g, t["lr"], (t["beta1"], t["beta2"])),
+                    make(self.arena_d, t["lr"] * t["lr_d_factor"], (t["d_beta1"], t["d_beta2"])))
         og = FlatAdam(self.arena_g, t["lr"], (t["beta1"], t["beta2"]))
         od = FlatAdam(self.arena_d, t["lr"] * t["lr_d_factor"], (t["d_beta1"], t["d_beta2"]))
         return og, od
