@@ -33,6 +33,238 @@ __device__ __forceinline__ float2 stats_of(float m, float s)            // (subt
 {
     return m == -INFINITY ? make_float2(0.f, s) : make_float2(m, 1.0f / s);      // s is 0 here, or a NaN
 }
+
+// ----------------------------------------------------------------------------- up to 16384 codes: a row in registers, read once
+// A team of TL lanes (a part of a wave), or of W whole waves (then TL = 64), holds one row: lane t the columns (j TL W + t) 4 .. + 3,
+// j < NJ.  The columns of a lane are the same for every row, so the sums over rows are registers too and the row's own maximum and sum
+// are the only things that cross lanes (shuffles; with W > 1 one LDS exchange and one barrier a row, the buffer alternating).  The next
+// row's loads are issued before the present row is worked on.
+template <typename T> struct Quad;
+template <> struct Quad<float> { typedef float4 type; };
+template <> struct Quad<uint16_t> { typedef ushort4 type; };
+template <> struct Quad<_Float16> { typedef ushort4 type; };
+__device__ __forceinline__ float widen(float v, float) { return v; }
+__device__ __forceinline__ float widen(uint16_t v, uint16_t) { return __uint_as_float((uint32_t)v << 16); }
+__device__ __forceinline__ float widen(uint16_t v, _Float16) { return (float)__builtin_bit_cast(_Float16, v); }
+
+// four columns from c; columns at and after E read as -inf.  VEC: rows start on the quad's alignment and E is a multiple of 4
+template <typename T, bool VEC>
+__device__ __forceinline__ void load4(const T *row, int c, int E, float (&x)[4])
+{
+    if (VEC) {
+        if (c < E) {
+            const typename Quad<T>::type q = *reinterpret_cast<const typename Quad<T>::type *>(row + c);
+            x[0] = widen(q.x, T()); x[1] = widen(q.y, T()); x[2] = widen(q.z, T()); x[3] = widen(q.w, T());
+        } else {
+            x[0] = x[1] = x[2] = x[3] = -INFINITY;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = c + i < E ? Ld<T>::get(row + c + i) : -INFINITY;
+    }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store4(T *row, int c, int E, const float (&x)[4])
+{
+    if (VEC) {
+        if (c < E) {
+            T q[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) Ld<T>::put(q + i, x[i]);
+            *reinterpret_cast<typename Quad<T>::type *>(row + c) = *reinterpret_cast<const typename Quad<T>::type *>(q);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (c + i < E) Ld<T>::put(row + c + i, x[i]);
+    }
+}
+template <int TL> __device__ __forceinline__ float team_max(float v)
+{
+    if (TL == 64) return wave_max(v);
+#pragma unroll
+    for (int o = TL / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+template <int TL> __device__ __forceinline__ float team_sum(float v)
+{
+    if (TL == 64) return wave_sum(v);
+#pragma unroll
+    for (int o = TL / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+template <typename T, int TL, int NJ, int W, bool VEC>
+__global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_fwd_kernel(const T *__restrict__ z, int64_t ld, const uint8_t *__restrict__ padded,
+                                                                          int64_t N, int E, float2 *__restrict__ stats, float *__restrict__ part)
+{
+    constexpr int TEAMS = W > 1 ? 1 : 256 / TL;                 // rows a block works on at a time
+    constexpr int SPAN = TL * W * 4;
+    __shared__ float2 ex[2][W];
+    extern __shared__ float cols[];                             // W == 1: the block's column sums
+    const int t = W > 1 ? threadIdx.x : threadIdx.x % TL;
+    const int64_t first = (int64_t)blockIdx.x * TEAMS + (W > 1 ? 0 : threadIdx.x / TL), step = (int64_t)gridDim.x * TEAMS;
+    float acc[NJ][4] = {}, x[NJ][4], y[NJ][4];
+    const auto fetch = [&](int64_t n, float (&v)[NJ][4]) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) load4<T, VEC>(z + n * ld, j * SPAN + t * 4, E, v[j]);
+    };
+    const auto next = [&](int64_t n) {                          // the row at or after n that is not padded
+        if (padded)
+            while (n < N && padded[n]) n += step;
+        return n;
+    };
+    int64_t n = next(first);
+    if (n < N) fetch(n, x);
+    int parity = 0;
+    while (n < N) {
+        const int64_t after = next(n + step);
+        if (after < N) fetch(after, y);
+        float m = -INFINITY, s = 0.f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = fmaxf(m, x[j][i]);
+        m = team_max<TL>(m);
+        const float m0 = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[j][i] = __expf(x[j][i] - m0);
+                s += x[j][i];
+            }
+        s = team_sum<TL>(s);
+        float M = m, S = s;
+        if (W > 1) {
+            if ((threadIdx.x & 63) == 0) ex[parity][threadIdx.x >> 6] = make_float2(m, s);
+            __syncthreads();
+            M = -INFINITY;
+            S = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) M = fmaxf(M, ex[parity][w].x);
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const float2 o = ex[parity][w];
+                S += o.y == 0.f ? 0.f : o.y * __expf(o.x - M);
+            }
+            parity ^= 1;
+        }
+        const float f = W > 1 ? (s == 0.f ? 0.f : __expf(m - M) / S) : (s == 0.f ? 0.f : 1.0f / s);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[j][i] = fmaf(x[j][i], f, acc[j][i]);
+        if (t == 0) stats[n] = stats_of(M, S);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[j][i] = y[j][i];
+        n = after;
+    }
+    float *out = part + (int64_t)blockIdx.x * E;
+    if (W > 1) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int c = j * SPAN + t * 4 + i;
+                if (c < E) out[c] = acc[j][i];
+            }
+        return;
+    }
+    if (TL < 64) {                                              // the teams of a wave, in an order of their own that never changes
+#pragma unroll
+        for (int o = 32; o >= TL; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[0][i] += __shfl_xor(acc[0][i], o, 64);
+    }
+    for (int w = 0; w < 4; ++w) {                               // then the waves, one after the other
+        if ((int)(threadIdx.x >> 6) == w && (threadIdx.x & 63) < TL) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int c = j * SPAN + t * 4 + i;
+                    if (c < E) cols[c] = w ? cols[c] + acc[j][i] : acc[j][i];
+                }
+        }
+        __syncthreads();
+    }
+    for (int c = threadIdx.x; c < E; c += 256) out[c] = cols[c];
+}
+
+template <typename T, int TL, int NJ, int W, bool VEC>
+__global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_grad_kernel(const T *__restrict__ z, int64_t ld, const uint8_t *__restrict__ padded,
+                                                                           int64_t N, int E, const float2 *__restrict__ stats,
+                                                                           const float *__restrict__ f, const float *__restrict__ sums,
+                                                                           const float *__restrict__ gout, T *__restrict__ dz)
+{
+    constexpr int TEAMS = W > 1 ? 1 : 256 / TL;
+    constexpr int SPAN = TL * W * 4;
+    __shared__ float ex[2][W];
+    const int t = W > 1 ? threadIdx.x : threadIdx.x % TL;
+    const int64_t step = (int64_t)gridDim.x * TEAMS;
+    int64_t n = (int64_t)blockIdx.x * TEAMS + (W > 1 ? 0 : threadIdx.x / TL);
+    float fr[NJ][4], x[NJ][4], y[NJ][4];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = j * SPAN + t * 4 + i;
+            fr[j][i] = c < E ? f[c] : 0.f;
+        }
+    const float scale = gout[0] * ((float)E / sums[2 * (int64_t)E]);
+    const auto fetch = [&](int64_t r, float (&v)[NJ][4]) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) load4<T, VEC>(z + r * ld, j * SPAN + t * 4, E, v[j]);
+    };
+    const auto skipped = [&](int64_t r) { return padded && padded[r]; };
+    if (n < N && !skipped(n)) fetch(n, x);
+    int parity = 0;
+    for (; n < N; n += step) {
+        const int64_t after = n + step;
+        if (after < N && !skipped(after)) fetch(after, y);
+        const bool none = skipped(n);
+        const float2 st = none ? make_float2(0.f, 0.f) : stats[n];
+        if (!none) {
+            float s = 0.f;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[j][i] = __expf(x[j][i] - st.x) * st.y;
+                    s = fmaf(fr[j][i], x[j][i], s);
+                }
+            s = team_sum<TL>(s);
+            if (W > 1) {
+                if ((threadIdx.x & 63) == 0) ex[parity][threadIdx.x >> 6] = s;
+                __syncthreads();
+                s = 0.f;
+#pragma unroll
+                for (int w = 0; w < W; ++w) s += ex[parity][w];
+                parity ^= 1;
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[j][i] = scale * x[j][i] * (fr[j][i] - s);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[j][i] = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) store4<T, VEC>(dz + n * E, j * SPAN + t * 4, E, x[j]);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[j][i] = y[j][i];
+    }
+}
+
+// ----------------------------------------------------------------------------- wider books: the row's statistics first, then column sums
 // block of 256: (m, s) pairs joined; red is 8 floats
 __device__ __forceinline__ float2 block_join(float m, float s, float *red)
 {
@@ -86,51 +318,46 @@ __global__ __launch_bounds__(256) void balance_cols_kernel(const T *__restrict__
     part[(int64_t)blockIdx.y * E + e] = a;
 }
 
-__global__ __launch_bounds__(256) void balance_zero_kernel(int *__restrict__ counts, int n)
-{
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i < n) counts[i] = 0;
-}
-// counts[0 .. E) and counts[E] = valid rows.  Whole numbers: the order of the additions does not show.
+// sums = {sum_n p_ne (E), counts (E), valid rows}: what data-parallel ranks add up before the loss is formed.  A block owns 32 columns: it adds
+// their partial sums (eight threads a column, in f64, joined in order) and reads all assignments for the ones that fall on them, which
+// costs 4 K / 32 bytes out of the L2 per score read and spares a zeroed histogram and its atomics.
+constexpr int BL_COLS = 32;
 template <typename I>
-__global__ __launch_bounds__(256) void balance_counts_kernel(const I *__restrict__ idx, const uint8_t *__restrict__ padded, int64_t N, int K, int E,
-                                                             int in_lds, int *__restrict__ counts)
-{
-    extern __shared__ int hist[];
-    if (in_lds) {
-        for (int e = threadIdx.x; e <= E; e += 256) hist[e] = 0;
-        __syncthreads();
-    }
-    int *to = in_lds ? hist : counts;
-    for (int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x; n < N; n += (int64_t)gridDim.x * 256) {
-        if (padded && padded[n]) continue;
-        atomicAdd(to + E, 1);
-        for (int k = 0; k < K; ++k) {
-            const int64_t e = (int64_t)idx[n * K + k];
-            if (e >= 0 && e < E) atomicAdd(to + e, 1);
-        }
-    }
-    if (in_lds) {
-        __syncthreads();
-        for (int e = threadIdx.x; e <= E; e += 256)
-            if (hist[e]) atomicAdd(counts + e, hist[e]);
-    }
-}
-
-// sums = {sum_n p_ne (E), counts (E), valid rows}: what data-parallel ranks add up before the loss is formed
-__global__ __launch_bounds__(256) void balance_sums_kernel(const float *__restrict__ part, int nparts, const int *__restrict__ counts, int E,
+__global__ __launch_bounds__(256) void balance_sums_kernel(const float *__restrict__ part, int nparts, const I *__restrict__ idx,
+                                                           const uint8_t *__restrict__ padded, int64_t N, int K, int E, int32_t *__restrict__ counts,
                                                            float *__restrict__ sums)
 {
-    const int e = blockIdx.x * 256 + threadIdx.x;
-    if (e > E) return;
-    if (e == E) {
-        sums[2 * (int64_t)E] = (float)counts[E];
-        return;
-    }
+    __shared__ double red[8][BL_COLS];
+    __shared__ int hist[BL_COLS + 1];
+    const int e0 = blockIdx.x * BL_COLS, c = threadIdx.x % BL_COLS, g = threadIdx.x / BL_COLS;
+    if (threadIdx.x <= BL_COLS) hist[threadIdx.x] = 0;
     double a = 0.0;
-    for (int i = 0; i < nparts; ++i) a += (double)part[(int64_t)i * E + e];
-    sums[e] = (float)a;
-    sums[E + e] = (float)counts[e];
+    if (e0 + c < E)
+        for (int i = g; i < nparts; i += 8) a += (double)part[(int64_t)i * E + e0 + c];
+    red[g][c] = a;
+    __syncthreads();
+    int valid = 0;
+    for (int64_t n = threadIdx.x; n < N; n += 256) {
+        if (padded && padded[n]) continue;
+        ++valid;
+        for (int k = 0; k < K; ++k) {
+            const int64_t e = (int64_t)idx[n * K + k] - e0;
+            if (e >= 0 && e < BL_COLS && e + e0 < E) atomicAdd(&hist[e], 1);
+        }
+    }
+    if (blockIdx.x == 0) atomicAdd(&hist[BL_COLS], valid);
+    __syncthreads();
+    if (g == 0 && e0 + c < E) {
+        double t = 0.0;
+        for (int i = 0; i < 8; ++i) t += red[i][c];
+        sums[e0 + c] = (float)t;
+        sums[E + e0 + c] = (float)hist[c];
+        counts[e0 + c] = hist[c];
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        sums[2 * (int64_t)E] = (float)hist[BL_COLS];
+        counts[E] = hist[BL_COLS];
+    }
 }
 
 __global__ __launch_bounds__(1024) void balance_final_kernel(const float *__restrict__ sums, int E, int K, float *__restrict__ loss, float *__restrict__ f)
@@ -180,15 +407,44 @@ __global__ __launch_bounds__(256) void balance_bwd_kernel(const T *__restrict__ 
 
 inline int64_t bl_chunks(int64_t n) { return n < 512 ? n : 512; }
 
+// How a row is held: the smallest team whose lanes hold it in at most 8 quads each.  wide: the kernels above
+struct BlForm {
+    int tl, nj, w;
+    bool wide;
+};
+inline BlForm bl_form(int E)
+{
+    const int q = (E + 3) / 4;                                  // quads of a row
+    if (q <= 4) return {4, 1, 1, false};
+    if (q <= 8) return {8, 1, 1, false};
+    if (q <= 16) return {16, 1, 1, false};
+    if (q <= 32) return {32, 1, 1, false};
+    if (q <= 64) return {64, 1, 1, false};
+    if (q <= 128) return {64, 2, 1, false};
+    if (q <= 256) return {64, 4, 1, false};
+    if (q <= 512) return {64, 8, 1, false};
+    if (q <= 1024) return {64, 4, 4, false};
+    if (q <= 2048) return {64, 4, 8, false};
+    if (q <= 4096) return {64, 4, 16, false};
+    return {0, 0, 0, true};
+}
+inline int bl_blocks(const BlForm &f, int64_t rows)
+{
+    const int64_t teams = f.w > 1 ? 1 : 256 / f.tl, most = f.w > 1 ? 256 * (16 / f.w) : 512;
+    const int64_t b = cdiv(rows, teams);
+    return (int)(b < most ? b : most);
+}
+
 }  // namespace mq
 
 using namespace mq;
 
-// statistics of the rows, then partial column sums
+// partial column sums
 extern "C" size_t mq_code_balance_workspace(int64_t rows, int codes)
 {
     if (rows <= 0 || codes <= 0) return 0;
-    return (size_t)bl_chunks(rows) * codes * sizeof(float);
+    const BlForm f = bl_form(codes);
+    return (size_t)(f.wide ? bl_chunks(rows) : bl_blocks(f, rows)) * codes * sizeof(float);
 }
 
 #define BL_TYPES(call)                                                    \
@@ -197,6 +453,48 @@ extern "C" size_t mq_code_balance_workspace(int64_t rows, int codes)
     case 1: call(uint16_t); break;                                        \
     default: call(_Float16); break;                                       \
     }
+// F(TL, NJ, W): one of the forms of bl_form
+#define BL_FORMS(F)                                                       \
+    if (f.tl == 4) F(4, 1, 1);                                            \
+    else if (f.tl == 8) F(8, 1, 1);                                       \
+    else if (f.tl == 16) F(16, 1, 1);                                     \
+    else if (f.tl == 32) F(32, 1, 1);                                     \
+    else if (f.w == 16) F(64, 4, 16);                                     \
+    else if (f.w == 8) F(64, 4, 8);                                       \
+    else if (f.w == 4) F(64, 4, 4);                                       \
+    else if (f.nj == 1) F(64, 1, 1);                                      \
+    else if (f.nj == 2) F(64, 2, 1);                                      \
+    else if (f.nj == 4) F(64, 4, 1);                                      \
+    else F(64, 8, 1);
+
+template <typename T>
+static void bl_forward(const T *z, int64_t ld, const uint8_t *padded, int64_t rows, int codes, float2 *st, float *part, const BlForm &f, int blocks, hipStream_t s)
+{
+    const bool vec = codes % 4 == 0 && ld % 4 == 0 && (uintptr_t)z % (4 * sizeof(T)) == 0;
+#define F(TL, NJ, W)                                                                                                                                  \
+    do {                                                                                                                                              \
+        const size_t lds = W > 1 ? 0 : (size_t)codes * sizeof(float);                                                                                 \
+        if (vec) hipLaunchKernelGGL((balance_fwd_kernel<T, TL, NJ, W, true>), dim3(blocks), dim3(W > 1 ? 64 * W : 256), lds, s, z, ld, padded, rows, codes, st, part); \
+        else hipLaunchKernelGGL((balance_fwd_kernel<T, TL, NJ, W, false>), dim3(blocks), dim3(W > 1 ? 64 * W : 256), lds, s, z, ld, padded, rows, codes, st, part);    \
+    } while (0)
+    BL_FORMS(F)
+#undef F
+}
+template <typename T>
+static void bl_backward(const T *z, int64_t ld, const uint8_t *padded, int64_t rows, int codes, const float2 *st, const float *fr, const float *sums, const float *gout, T *dz,
+                        const BlForm &f, hipStream_t s)
+{
+    const bool vec = codes % 4 == 0 && ld % 4 == 0 && ((uintptr_t)z | (uintptr_t)dz) % (4 * sizeof(T)) == 0;
+    const int64_t teams = f.w > 1 ? 1 : 256 / f.tl, want = cdiv(rows, teams), most = f.w > 1 ? 256 * (32 / f.w) : 2048;
+    const dim3 grid((unsigned)(want < most ? want : most));
+#define F(TL, NJ, W)                                                                                                                                  \
+    do {                                                                                                                                              \
+        if (vec) hipLaunchKernelGGL((balance_grad_kernel<T, TL, NJ, W, true>), grid, dim3(W > 1 ? 64 * W : 256), 0, s, z, ld, padded, rows, codes, st, fr, sums, gout, dz); \
+        else hipLaunchKernelGGL((balance_grad_kernel<T, TL, NJ, W, false>), grid, dim3(W > 1 ? 64 * W : 256), 0, s, z, ld, padded, rows, codes, st, fr, sums, gout, dz);    \
+    } while (0)
+    BL_FORMS(F)
+#undef F
+}
 
 extern "C" int mq_code_balance_sums(const void *logits, int dtype, int64_t row_stride, const void *idx, int idx64, int per_row, const uint8_t *padded,
                                     int64_t rows, int codes, void *stats, int32_t *counts, float *sums, void *workspace, size_t workspace_bytes,
@@ -211,23 +509,28 @@ extern "C" int mq_code_balance_sums(const void *logits, int dtype, int64_t row_s
                mq_code_balance_workspace(rows, codes));
     float *part = reinterpret_cast<float *>(workspace);
     float2 *st = reinterpret_cast<float2 *>(stats);
-    const int64_t chunk = cdiv(rows, bl_chunks(rows));
-    const int nparts = (int)cdiv(rows, chunk);
+    const BlForm f = bl_form(codes);
+    int nparts;
+    if (f.wide) {
+        const int64_t chunk = cdiv(rows, bl_chunks(rows));
+        nparts = (int)cdiv(rows, chunk);
 #define CALL(T)                                                                                                                                       \
     hipLaunchKernelGGL(balance_rows_kernel<T>, dim3((unsigned)rows), dim3(256), 0, S(stream), reinterpret_cast<const T *>(logits), row_stride, padded, codes, st); \
     hipLaunchKernelGGL(balance_cols_kernel<T>, dim3((unsigned)cdiv(codes, 256), nparts), dim3(256), 0, S(stream), reinterpret_cast<const T *>(logits), row_stride, padded, \
                        rows, codes, chunk, st, part)
-    BL_TYPES(CALL)
+        BL_TYPES(CALL)
 #undef CALL
-    hipLaunchKernelGGL(balance_zero_kernel, dim3((unsigned)cdiv(codes + 1, 256)), dim3(256), 0, S(stream), counts, codes + 1);
-    const int in_lds = codes < 16384;                               // 64 KiB of the 160 a compute unit has
-    const unsigned nb = (unsigned)(cdiv(rows, 256) < 256 ? cdiv(rows, 256) : 256);
-    const size_t lds = in_lds ? (size_t)(codes + 1) * sizeof(int) : 0;
+    } else {
+        nparts = bl_blocks(f, rows);
+#define CALL(T) bl_forward(reinterpret_cast<const T *>(logits), row_stride, padded, rows, codes, st, part, f, nparts, S(stream))
+        BL_TYPES(CALL)
+#undef CALL
+    }
+    const dim3 grid((unsigned)cdiv(codes, BL_COLS));
     if (idx64)
-        hipLaunchKernelGGL(balance_counts_kernel<int64_t>, dim3(nb), dim3(256), lds, S(stream), reinterpret_cast<const int64_t *>(idx), padded, rows, per_row, codes, in_lds, counts);
+        hipLaunchKernelGGL(balance_sums_kernel<int64_t>, grid, dim3(256), 0, S(stream), part, nparts, reinterpret_cast<const int64_t *>(idx), padded, rows, per_row, codes, counts, sums);
     else
-        hipLaunchKernelGGL(balance_counts_kernel<int32_t>, dim3(nb), dim3(256), lds, S(stream), reinterpret_cast<const int32_t *>(idx), padded, rows, per_row, codes, in_lds, counts);
-    hipLaunchKernelGGL(balance_sums_kernel, dim3((unsigned)cdiv(codes + 1, 256)), dim3(256), 0, S(stream), part, nparts, counts, codes, sums);
+        hipLaunchKernelGGL(balance_sums_kernel<int32_t>, grid, dim3(256), 0, S(stream), part, nparts, reinterpret_cast<const int32_t *>(idx), padded, rows, per_row, codes, counts, sums);
     MQ_LAUNCH_CHECK("mq_code_balance_sums");
     return 0;
 }
@@ -247,11 +550,18 @@ extern "C" int mq_code_balance_bwd(const void *logits, int dtype, int64_t row_st
     MQ_REQUIRE(dtype >= 0 && dtype <= 2, "mq_code_balance_bwd: dtype %d (0 f32, 1 bf16, 2 f16)", dtype);
     MQ_REQUIRE(rows > 0 && rows < INT32_MAX && codes > 0 && row_stride >= codes, "mq_code_balance_bwd: bad sizes");
     const float2 *st = reinterpret_cast<const float2 *>(stats);
+    const BlForm form = bl_form(codes);
+    if (form.wide) {
 #define CALL(T)                                                                                                                                       \
     hipLaunchKernelGGL(balance_bwd_kernel<T>, dim3((unsigned)rows), dim3(256), 0, S(stream), reinterpret_cast<const T *>(logits), row_stride, padded, codes, st, fractions, \
                        sums, gout, reinterpret_cast<T *>(dlogits))
-    BL_TYPES(CALL)
+        BL_TYPES(CALL)
 #undef CALL
+    } else {
+#define CALL(T) bl_backward(reinterpret_cast<const T *>(logits), row_stride, padded, rows, codes, st, fractions, sums, gout, reinterpret_cast<T *>(dlogits), form, S(stream))
+        BL_TYPES(CALL)
+#undef CALL
+    }
     MQ_LAUNCH_CHECK("mq_code_balance_bwd");
     return 0;
 }
