@@ -660,14 +660,14 @@ int mq_comm_destroy(mqComm *comm);
  * Balance loss: p_n = softmax(z_n), P = mean of p_n over the Nv valid rows, f_e = counts_e / (Nv K) from the K assignments of every
  * valid row (idx (rows, K) int32, or int64 with idx64 = 1; an index outside [0, codes) is not counted);  L = codes * sum_e f_e P_e;
  * dL/dz_ne = gout * codes / Nv * p_ne * (f_e - sum_j f_j p_nj), 0 on padded rows.  No valid row: L = 0.
- *   sums     leaves {sum_n p_ne (codes), counts (codes), Nv} in sums (2 codes + 1 floats; data-parallel ranks add these up), the counts in
- *            counts (codes + 1 int32, the last one Nv), and per-row statistics (2 floats a row) for bwd
- *   final    the loss (1 float) and f (codes floats) from the sums
+ *   fwd      leaves {sum_n p_ne (codes), counts (codes), Nv} in sums (2 codes + 1 floats), the counts in counts (codes int32) and per-row
+ *            statistics (2 floats a row) for bwd; with loss and fractions not NULL it goes on to `final`
+ *   final    the loss (1 float) and f (codes floats) from sums that data-parallel ranks have added up
  *   bwd      dlogits (rows, codes) dense, of the scores' dtype */
-size_t mq_code_balance_workspace(int64_t rows, int codes);
-int mq_code_balance_sums(const void *logits, int dtype, int64_t row_stride, const void *idx, int idx64, int per_row,
-                         const uint8_t *padded, int64_t rows, int codes, void *stats, int32_t *counts, float *sums, void *workspace,
-                         size_t workspace_bytes, mqStream stream);
+size_t mq_code_balance_workspace(int64_t rows, int codes, int dtype);
+int mq_code_balance_fwd(const void *logits, int dtype, int64_t row_stride, const void *idx, int idx64, int per_row,
+                        const uint8_t *padded, int64_t rows, int codes, void *stats, int32_t *counts, float *sums, float *loss,
+                        float *fractions, void *workspace, size_t workspace_bytes, mqStream stream);
 int mq_code_balance_final(const float *sums, int codes, int per_row, float *loss, float *fractions, mqStream stream);
 int mq_code_balance_bwd(const void *logits, int dtype, int64_t row_stride, const uint8_t *padded, int64_t rows, int codes,
                         const void *stats, const float *sums, const float *fractions, const float *gout, void *dlogits, mqStream stream);

@@ -19,6 +19,7 @@
 namespace mq {
 
 constexpr int AW_CHUNK = 4096;        // elements a block updates: four groups a wave
+constexpr int AW_NORM = 4;            // chunks a block of the norm reads
 constexpr int AW_GRADS = 460;         // gradient addresses a launch carries by value (kernel arguments hold 4 KiB)
 
 struct AwRow {                        // one tensor; the layout of the table is private to this file
@@ -39,7 +40,7 @@ struct AwControl {                    // start of the control buffer; AwState pe
 };
 struct AwState {
     int step;
-    float step_size, inv_bc2, keep;   // lr / (1 - b1^t), 1 / sqrt(1 - b2^t), 1 - lr wd
+    float step_size, inv_bc2, keep;   // lr / (1 - b1^t), 1 / sqrt(1 - b2^t), 1 - lr wd (1 where nothing decays)
 };
 struct AwGrads {
     uint64_t g[AW_GRADS];             // address | element type << 62; 0: no gradient
@@ -91,32 +92,42 @@ __device__ __forceinline__ double wave_sum_f64(double v)
     return v;
 }
 
-// Squares in f64: a gradient of 1e20 has a norm, and the sum's order (lane, wave, block) costs nothing in f32 terms.
+// Squares in f64: a gradient of 1e20 has a norm, and the sum's order (lane, wave, block) costs nothing in f32 terms.  A block takes
+// AW_NORM of the update's chunks, whose rows it looks up together: with one chunk a block the look-ups' latency was half of the time.
 __global__ __launch_bounds__(256) void adamw_sumsq_kernel(const AwGrads grads, const AwRow *__restrict__ rows, const int *__restrict__ row_of,
-                                                          int row0, int block0, double *__restrict__ part)
+                                                          int row0, int block0, int nb, int part0, double *__restrict__ part)
 {
     __shared__ double red[4];
-    const int r = row_of[block0 + blockIdx.x];
-    const uint64_t tagged = grads.g[r - row0];
-    double s = 0.0;
-    if (tagged) {
-        const int64_t n = rows[r].n;
-        const int64_t e0 = (int64_t)(block0 + (int)blockIdx.x - rows[r].first_block) * AW_CHUNK + threadIdx.x * 4;
+    const int b0 = blockIdx.x * AW_NORM;
+    int r[AW_NORM];
+    uint64_t tagged[AW_NORM];
+    int64_t n[AW_NORM], e0[AW_NORM];
+#pragma unroll
+    for (int c = 0; c < AW_NORM; ++c) r[c] = row_of[block0 + (b0 + c < nb ? b0 + c : nb - 1)];
+#pragma unroll
+    for (int c = 0; c < AW_NORM; ++c) {
+        tagged[c] = grads.g[r[c] - row0];
+        n[c] = b0 + c < nb && tagged[c] ? rows[r[c]].n : 0;        // 0: nothing is read
+        e0[c] = (int64_t)(block0 + b0 + c - rows[r[c]].first_block) * AW_CHUNK + threadIdx.x * 4;
+    }
+    double s = 0.0, u = 0.0;
+#pragma unroll
+    for (int c = 0; c < AW_NORM; ++c) {
         float4 g[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) g[k] = aw_grad4(tagged, e0 + k * 1024, n);
+        for (int k = 0; k < 4; ++k) g[k] = aw_grad4(tagged[c], e0[c] + k * 1024, n[c]);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             s = fma((double)g[k].x, (double)g[k].x, s);
-            s = fma((double)g[k].y, (double)g[k].y, s);
+            u = fma((double)g[k].y, (double)g[k].y, u);
             s = fma((double)g[k].z, (double)g[k].z, s);
-            s = fma((double)g[k].w, (double)g[k].w, s);
+            u = fma((double)g[k].w, (double)g[k].w, u);
         }
     }
-    s = wave_sum_f64(s);
+    s = wave_sum_f64(s + u);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) part[block0 + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+    if (threadIdx.x == 0) part[part0 + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 // One block: the norm from the partial sums (first launch of a call), then every tensor's step count and the factors that go with it.
@@ -185,30 +196,61 @@ __device__ __forceinline__ uint32_t wave_pk_max(uint32_t v)
     return pk_max(pk_max(a, b), pk_max(c, d));
 }
 __device__ __forceinline__ uint32_t mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-__device__ __forceinline__ uint32_t exp_finite(float x)
-{
-    const uint32_t b = mag(x);
-    return b < 0x7f800000u ? b >> 23 : 0u;
-}
-// base from the group's largest finite exponent: the binade above it is the topmost of 2^EB
+// base from the group's largest exponent: the binade above it is the topmost of 2^EB
 template <int EB>
 __device__ __forceinline__ uint32_t base_of(uint32_t e)
 {
     const int b = (int)e + 1 - ((1 << EB) - 1);
     return b > 0 ? (uint32_t)b : 0u;
 }
-// add: what goes under the kept bits (16 random bits << 4, or the round-to-nearest-even term)
+// code of one element; add: what goes under the kept bits (16 random bits << 4, or the round-to-nearest-even term)
 template <int EB>
-__device__ __forceinline__ uint32_t encode8(float x, uint32_t base, uint32_t add)
+__device__ __forceinline__ uint32_t code8(float x, uint32_t base, uint32_t add)
 {
-    constexpr int most = 1 << (EB + 3);
     const uint32_t b = mag(x);
-    int c = (int)((b + add) >> 20) - (int)(8 * base);
-    if (c < 1) c = (EB == 5 && b > 0) ? 1 : 0;
-    if (b >= 0x7f800000u) c = b == 0x7f800000u ? most - 2 : most - 1;
-    uint32_t u = (uint32_t)c;
-    if (EB == 4 && c > 0) u |= (__float_as_uint(x) >> 24) & 0x80u;
+    const int c = (int)(b - (base << 23) + add) >> 20;             // code 1 starts at (8 base + 1) << 20
+    const uint32_t u = (uint32_t)max(c, EB == 5 ? (int)min(b, 1u) : 0);
+    if (EB == 4) return u | (u ? (__float_as_uint(x) >> 24) & 0x80u : 0u);
     return u;
+}
+template <int EB>
+__device__ __forceinline__ uint32_t special8(float x)               // of infinity and NaN
+{
+    constexpr uint32_t most = 1u << (EB + 3);
+    const uint32_t c = mag(x) == 0x7f800000u ? most - 2 : most - 1;
+    return EB == 4 ? c | ((__float_as_uint(x) >> 24) & 0x80u) : c;
+}
+// Four elements to a word of codes; `top`: the largest exponent of the group, 255 where something in it is infinite or NaN.  Then the base is
+// that of the finite ones and the others get their special codes: a branch the whole wave takes or leaves.
+template <int EB, typename ADD>
+__device__ __forceinline__ uint32_t word8(const float4 &x, uint32_t base, bool specials, ADD add)
+{
+    uint32_t c[4] = {code8<EB>(x.x, base, add(x.x, 0)), code8<EB>(x.y, base, add(x.y, 1)), code8<EB>(x.z, base, add(x.z, 2)), code8<EB>(x.w, base, add(x.w, 3))};
+    if (specials) {
+        if (mag(x.x) >= 0x7f800000u) c[0] = special8<EB>(x.x);
+        if (mag(x.y) >= 0x7f800000u) c[1] = special8<EB>(x.y);
+        if (mag(x.z) >= 0x7f800000u) c[2] = special8<EB>(x.z);
+        if (mag(x.w) >= 0x7f800000u) c[3] = special8<EB>(x.w);
+    }
+    return c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
+}
+__device__ __forceinline__ uint32_t exponent_max(const float4 &x) { return max(max(mag(x.x), mag(x.y)), max(mag(x.z), mag(x.w))) >> 23; }
+__device__ __forceinline__ uint32_t finite_mag(float x)
+{
+    const uint32_t b = mag(x);
+    return b < 0x7f800000u ? b : 0u;
+}
+__device__ __forceinline__ uint32_t exponent_max_finite(const float4 &x)
+{
+    return max(max(finite_mag(x.x), finite_mag(x.y)), max(finite_mag(x.z), finite_mag(x.w))) >> 23;
+}
+// the group's two exponents (m in the low half); specials: whether anything in it is infinite or NaN
+__device__ __forceinline__ uint32_t group_top(const float4 &m, const float4 &v, bool &specials)
+{
+    uint32_t top = wave_pk_max(exponent_max(m) | exponent_max(v) << 16);
+    specials = (top & 0xffffu) == 255u || top >> 16 == 255u;
+    if (specials) top = wave_pk_max(exponent_max_finite(m) | exponent_max_finite(v) << 16);
+    return top;
 }
 template <int EB>
 __device__ __forceinline__ float decode8(uint32_t u, uint32_t base)
@@ -216,19 +258,44 @@ __device__ __forceinline__ float decode8(uint32_t u, uint32_t base)
     constexpr uint32_t most = 1u << (EB + 3);
     const uint32_t c = u & (most - 1);
     uint32_t b = c ? (c + 8 * base) << 20 : 0u;
-    if (c >= most - 2) b = c == most - 2 ? 0x7f800000u : 0x7fc00000u;
     if (EB == 4) b |= (u & 0x80u) << 24;
     return __uint_as_float(b);
 }
+template <int EB>
+__device__ __forceinline__ float decode8_special(uint32_t u, uint32_t base)
+{
+    constexpr uint32_t most = 1u << (EB + 3);
+    const uint32_t c = u & (most - 1);
+    if (c < most - 2) return decode8<EB>(u, base);
+    return __uint_as_float((c == most - 2 ? 0x7f800000u : 0x7fc00000u) | (EB == 4 ? (u & 0x80u) << 24 : 0u));
+}
+// whether one of the word's four codes is a special one (its bits 1 .. all set): a byte of t is 0 where it is
+template <int EB>
+__device__ __forceinline__ bool any_special(uint32_t w)
+{
+    const uint32_t t = ~w & (EB == 4 ? 0x7e7e7e7eu : 0xfefefefeu);
+    return ((t - 0x01010101u) & ~t & 0x80808080u) != 0u;
+}
+template <int EB>
+__device__ __forceinline__ float4 unword8(uint32_t w, uint32_t base, bool specials)
+{
+    if (specials)
+        return make_float4(decode8_special<EB>(w & 255, base), decode8_special<EB>((w >> 8) & 255, base), decode8_special<EB>((w >> 16) & 255, base), decode8_special<EB>(w >> 24, base));
+    return make_float4(decode8<EB>(w & 255, base), decode8<EB>((w >> 8) & 255, base), decode8<EB>((w >> 16) & 255, base), decode8<EB>(w >> 24, base));
+}
 __device__ __forceinline__ uint32_t nearest_add(float x) { return 0x7ffffu + ((mag(x) >> 20) & 1u); }
 
+// Blocks run from the last chunk to the first: the norm has just read the gradients in order, so the last of them are still in the
+// 256 MB cache.  Root and reciprocal are the hardware's (one ulp each); v is held up to the smallest normal number under the root,
+// which the hardware needs, so with eps = 0 an element that never had a gradient stays put instead of becoming 0 / 0.
 template <bool Q8>
 __global__ __launch_bounds__(256) void adamw_kernel(const AwGrads grads, const AwRow *__restrict__ rows, const int *__restrict__ row_of, int row0,
                                                     int block0, const AwHyper h, const AwControl *__restrict__ ctl,
                                                     const AwState *__restrict__ st)
 {
 #pragma clang fp contract(off)
-    const int r = row_of[block0 + blockIdx.x];
+    const int block = block0 + (int)(gridDim.x - 1 - blockIdx.x);
+    const int r = row_of[block];
     const uint64_t tagged = grads.g[r - row0];
     if (!tagged) return;                                            // no gradient this step: the tensor stays as it is
     const AwRow row = rows[r];
@@ -237,11 +304,12 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AwGrads grads, const A
     const uint32_t k0 = ctl->k0, k1 = ctl->k1;
     const int64_t n = row.n;
     const int64_t room = (n + 255) & ~(int64_t)255;                 // the moments' layout is padded to whole groups
-    const int64_t e0 = (int64_t)(block0 + (int)blockIdx.x - row.first_block) * AW_CHUNK + threadIdx.x * 4;
+    const int64_t e0 = (int64_t)(block - row.first_block) * AW_CHUNK + threadIdx.x * 4;
     const bool pvec = ((uintptr_t)row.p & 15) == 0;
     const float *m32 = reinterpret_cast<const float *>(row.m), *v32 = reinterpret_cast<const float *>(row.v);
     const uint32_t *m8 = reinterpret_cast<const uint32_t *>(row.m), *v8 = reinterpret_cast<const uint32_t *>(row.v);
     float4 p[4], g[4], m[4], v[4];
+    uint32_t mc[4], vc[4], mb[4], vb[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const int64_t e = e0 + k * 1024;
@@ -249,9 +317,10 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AwGrads grads, const A
         g[k] = aw_grad4(tagged, e, n);
         p[k] = aw_load4(row.p, e, n, pvec);
         if (Q8) {
-            const uint32_t mc = m8[e >> 2], vc = v8[e >> 2], mb = row.mb[e >> 8], vb = row.vb[e >> 8];
-            m[k] = make_float4(decode8<4>(mc & 255, mb), decode8<4>((mc >> 8) & 255, mb), decode8<4>((mc >> 16) & 255, mb), decode8<4>(mc >> 24, mb));
-            v[k] = make_float4(decode8<5>(vc & 255, vb), decode8<5>((vc >> 8) & 255, vb), decode8<5>((vc >> 16) & 255, vb), decode8<5>(vc >> 24, vb));
+            mc[k] = m8[e >> 2];
+            vc[k] = v8[e >> 2];
+            mb[k] = row.mb[e >> 8];
+            vb[k] = row.vb[e >> 8];
         } else {
             m[k] = *reinterpret_cast<const float4 *>(m32 + e);
             v[k] = *reinterpret_cast<const float4 *>(v32 + e);
@@ -261,12 +330,18 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AwGrads grads, const A
         gi *= coef;
         mi = mi + (gi - mi) * h.omb1;
         vi = vi * h.b2 + h.omb2 * gi * gi;
-        pi = pi * s.keep - s.step_size * (mi / (sqrtf(vi) * s.inv_bc2 + h.eps));
+        const float denom = __builtin_amdgcn_sqrtf(vi < 1.17549435e-38f ? 1.17549435e-38f : vi) * s.inv_bc2 + h.eps;      // a NaN stays
+        pi = pi * s.keep - s.step_size * (mi * __builtin_amdgcn_rcpf(denom));
     };
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const int64_t e = e0 + k * 1024;
         if (e >= room) continue;
+        if (Q8) {
+            const bool held = __builtin_amdgcn_ballot_w64(any_special<4>(mc[k]) || any_special<5>(vc[k])) != 0;
+            m[k] = unword8<4>(mc[k], mb[k], held);
+            v[k] = unword8<5>(vc[k], vb[k], held);
+        }
         one(p[k].x, g[k].x, m[k].x, v[k].x);
         one(p[k].y, g[k].y, m[k].y, v[k].y);
         one(p[k].z, g[k].z, m[k].z, v[k].z);
@@ -280,23 +355,18 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AwGrads grads, const A
             if (e + 3 < n) row.p[e + 3] = p[k].w;
         }
         if (Q8) {
-            const uint32_t em = max(max(exp_finite(m[k].x), exp_finite(m[k].y)), max(exp_finite(m[k].z), exp_finite(m[k].w)));
-            const uint32_t ev = max(max(exp_finite(v[k].x), exp_finite(v[k].y)), max(exp_finite(v[k].z), exp_finite(v[k].w)));
-            const uint32_t top = wave_pk_max(em | (ev << 16));
-            const uint32_t mb = base_of<4>(top & 0xffffu), vb = base_of<5>(top >> 16);
+            bool specials;
+            const uint32_t top = group_top(m[k], v[k], specials);
+            const uint32_t mbase = base_of<4>(top & 0xffffu), vbase = base_of<5>(top >> 16);
             const uint64_t at = (uint64_t)(row.position + e);
             uint32_t w[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = mix32((((uint32_t)at + j) ^ k0) + (uint32_t)(at >> 32) * 0x9E3779B1u) + k1;
-            const uint32_t mc = encode8<4>(m[k].x, mb, (w[0] >> 16) << 4) | encode8<4>(m[k].y, mb, (w[1] >> 16) << 4) << 8 |
-                                encode8<4>(m[k].z, mb, (w[2] >> 16) << 4) << 16 | encode8<4>(m[k].w, mb, (w[3] >> 16) << 4) << 24;
-            const uint32_t vc = encode8<5>(v[k].x, vb, (w[0] & 0xffffu) << 4) | encode8<5>(v[k].y, vb, (w[1] & 0xffffu) << 4) << 8 |
-                                encode8<5>(v[k].z, vb, (w[2] & 0xffffu) << 4) << 16 | encode8<5>(v[k].w, vb, (w[3] & 0xffffu) << 4) << 24;
-            reinterpret_cast<uint32_t *>(row.m)[e >> 2] = mc;
-            reinterpret_cast<uint32_t *>(row.v)[e >> 2] = vc;
+            reinterpret_cast<uint32_t *>(row.m)[e >> 2] = word8<4>(m[k], mbase, specials, [&](float, int j) { return (w[j] >> 16) << 4; });
+            reinterpret_cast<uint32_t *>(row.v)[e >> 2] = word8<5>(v[k], vbase, specials, [&](float, int j) { return (w[j] & 0xffffu) << 4; });
             if ((threadIdx.x & 63) == 0) {
-                row.mb[e >> 8] = (uint8_t)mb;
-                row.vb[e >> 8] = (uint8_t)vb;
+                row.mb[e >> 8] = (uint8_t)mbase;
+                row.vb[e >> 8] = (uint8_t)vbase;
             }
         } else {
             *reinterpret_cast<float4 *>(reinterpret_cast<float *>(row.m) + e) = m[k];
@@ -314,14 +384,11 @@ __global__ __launch_bounds__(256) void moments8_encode_kernel(const float *__res
     if (grp >= groups) return;
     const int64_t at = grp * 64 + (threadIdx.x & 63);
     const float4 a = reinterpret_cast<const float4 *>(m)[at], b = reinterpret_cast<const float4 *>(v)[at];
-    const uint32_t em = max(max(exp_finite(a.x), exp_finite(a.y)), max(exp_finite(a.z), exp_finite(a.w)));
-    const uint32_t ev = max(max(exp_finite(b.x), exp_finite(b.y)), max(exp_finite(b.z), exp_finite(b.w)));
-    const uint32_t top = wave_pk_max(em | (ev << 16));
+    bool specials;
+    const uint32_t top = group_top(a, b, specials);
     const uint32_t bm = base_of<4>(top & 0xffffu), bv = base_of<5>(top >> 16);
-    mc[at] = encode8<4>(a.x, bm, nearest_add(a.x)) | encode8<4>(a.y, bm, nearest_add(a.y)) << 8 |
-             encode8<4>(a.z, bm, nearest_add(a.z)) << 16 | encode8<4>(a.w, bm, nearest_add(a.w)) << 24;
-    vc[at] = encode8<5>(b.x, bv, nearest_add(b.x)) | encode8<5>(b.y, bv, nearest_add(b.y)) << 8 |
-             encode8<5>(b.z, bv, nearest_add(b.z)) << 16 | encode8<5>(b.w, bv, nearest_add(b.w)) << 24;
+    mc[at] = word8<4>(a, bm, specials, [](float x, int) { return nearest_add(x); });
+    vc[at] = word8<5>(b, bv, specials, [](float x, int) { return nearest_add(x); });
     if ((threadIdx.x & 63) == 0) {
         mb[grp] = (uint8_t)bm;
         vb[grp] = (uint8_t)bv;
@@ -338,21 +405,17 @@ __global__ __launch_bounds__(256) void moments8_decode_kernel(const uint2 *__res
     if (i >= n8) return;
     const uint2 a = mc[i], b = vc[i];
     const uint32_t bm = mb[i >> 5], bv = vb[i >> 5];
-    float x[8], y[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        x[j] = decode8<4>(((j < 4 ? a.x : a.y) >> (8 * (j & 3))) & 255u, bm);
-        y[j] = decode8<5>(((j < 4 ? b.x : b.y) >> (8 * (j & 3))) & 255u, bv);
-    }
+    const bool held = __builtin_amdgcn_ballot_w64(any_special<4>(a.x) || any_special<4>(a.y) || any_special<5>(b.x) || any_special<5>(b.y)) != 0;
+    const float4 x0 = unword8<4>(a.x, bm, held), x1 = unword8<4>(a.y, bm, held), y0 = unword8<5>(b.x, bv, held), y1 = unword8<5>(b.y, bv, held);
     if (BF16) {
         const auto two = [](float lo, float hi) { return (__float_as_uint(lo) >> 16) | (__float_as_uint(hi) & 0xffff0000u); };
-        reinterpret_cast<uint4 *>(m)[i] = make_uint4(two(x[0], x[1]), two(x[2], x[3]), two(x[4], x[5]), two(x[6], x[7]));
-        reinterpret_cast<uint4 *>(v)[i] = make_uint4(two(y[0], y[1]), two(y[2], y[3]), two(y[4], y[5]), two(y[6], y[7]));
+        reinterpret_cast<uint4 *>(m)[i] = make_uint4(two(x0.x, x0.y), two(x0.z, x0.w), two(x1.x, x1.y), two(x1.z, x1.w));
+        reinterpret_cast<uint4 *>(v)[i] = make_uint4(two(y0.x, y0.y), two(y0.z, y0.w), two(y1.x, y1.y), two(y1.z, y1.w));
     } else {
-        reinterpret_cast<float4 *>(m)[2 * i] = make_float4(x[0], x[1], x[2], x[3]);
-        reinterpret_cast<float4 *>(m)[2 * i + 1] = make_float4(x[4], x[5], x[6], x[7]);
-        reinterpret_cast<float4 *>(v)[2 * i] = make_float4(y[0], y[1], y[2], y[3]);
-        reinterpret_cast<float4 *>(v)[2 * i + 1] = make_float4(y[4], y[5], y[6], y[7]);
+        reinterpret_cast<float4 *>(m)[2 * i] = x0;
+        reinterpret_cast<float4 *>(m)[2 * i + 1] = x1;
+        reinterpret_cast<float4 *>(v)[2 * i] = y0;
+        reinterpret_cast<float4 *>(v)[2 * i + 1] = y1;
     }
 }
 
@@ -441,6 +504,7 @@ extern "C" int mq_adamw_step(const mqAdamwDesc *d, const int64_t *numel_host, co
     h.seed = d->seed;
     double *part = reinterpret_cast<double *>(workspace);
     // three passes over the launches of up to AW_GRADS tensors: squares, factors, update
+    int parts = 0;
     for (int pass = d->max_norm > 0 ? 0 : 1; pass < 3; ++pass) {
         int block0 = 0;
         for (int row0 = 0; row0 < n; row0 += AW_GRADS) {
@@ -453,10 +517,12 @@ extern "C" int mq_adamw_step(const mqAdamwDesc *d, const int64_t *numel_host, co
                 nb += (int)aw_blocks(numel_host[row0 + i]);
             }
             if (pass == 1)
-                hipLaunchKernelGGL(adamw_prepare_kernel, dim3(1), dim3(1024), 0, S(stream), g, rows, row0, nr, row0 == 0, part, d->max_norm > 0 ? blocks : 0, h, ctl, st);
-            else if (nb && pass == 0)
-                hipLaunchKernelGGL(adamw_sumsq_kernel, dim3(nb), dim3(256), 0, S(stream), g, rows, row_of, row0, block0, part);
-            else if (nb && d->state_bits == 8)
+                hipLaunchKernelGGL(adamw_prepare_kernel, dim3(1), dim3(1024), 0, S(stream), g, rows, row0, nr, row0 == 0, part, parts, h, ctl, st);
+            else if (nb && pass == 0) {
+                const int np = (int)cdiv(nb, AW_NORM);
+                hipLaunchKernelGGL(adamw_sumsq_kernel, dim3(np), dim3(256), 0, S(stream), g, rows, row_of, row0, block0, nb, parts, part);
+                parts += np;
+            } else if (nb && d->state_bits == 8)
                 hipLaunchKernelGGL(adamw_kernel<true>, dim3(nb), dim3(256), 0, S(stream), g, rows, row_of, row0, block0, h, ctl, st);
             else if (nb)
                 hipLaunchKernelGGL(adamw_kernel<false>, dim3(nb), dim3(256), 0, S(stream), g, rows, row_of, row0, block0, h, ctl, st);

@@ -34,48 +34,70 @@ __device__ __forceinline__ float2 stats_of(float m, float s)            // (subt
     return m == -INFINITY ? make_float2(0.f, s) : make_float2(m, 1.0f / s);      // s is 0 here, or a NaN
 }
 
-// ----------------------------------------------------------------------------- up to 16384 codes: a row in registers, read once
-// A team of TL lanes (a part of a wave), or of W whole waves (then TL = 64), holds one row: lane t the columns (j TL W + t) 4 .. + 3,
-// j < NJ.  The columns of a lane are the same for every row, so the sums over rows are registers too and the row's own maximum and sum
-// are the only things that cross lanes (shuffles; with W > 1 one LDS exchange and one barrier a row, the buffer alternating).  The next
-// row's loads are issued before the present row is worked on.
-template <typename T> struct Quad;
-template <> struct Quad<float> { typedef float4 type; };
-template <> struct Quad<uint16_t> { typedef ushort4 type; };
-template <> struct Quad<_Float16> { typedef ushort4 type; };
-__device__ __forceinline__ float widen(float v, float) { return v; }
-__device__ __forceinline__ float widen(uint16_t v, uint16_t) { return __uint_as_float((uint32_t)v << 16); }
-__device__ __forceinline__ float widen(uint16_t v, _Float16) { return (float)__builtin_bit_cast(_Float16, v); }
-
-// four columns from c; columns at and after E read as -inf.  VEC: rows start on the quad's alignment and E is a multiple of 4
-template <typename T, bool VEC>
-__device__ __forceinline__ void load4(const T *row, int c, int E, float (&x)[4])
+// ----------------------------------------------------------------------------- a row in registers, read once
+// A team of TL lanes (a part of a wave), or of W whole waves (then TL = 64), holds one row as NQ quads of 16 bytes a lane: lane t the
+// columns (j TL W + t) EPQ .. + EPQ - 1, j < NQ.  The columns of a lane are the same for every row, so the sums over rows are registers too
+// and the row's own maximum and sum are the only things that cross lanes (shuffles; with W > 1 one LDS exchange and one barrier a row,
+// the buffer alternating).  Two rows are in flight behind the one that is worked on, as they lie in memory (bf16 takes half the registers);
+// what says whether a row is padded is read one row further ahead, so that no load waits for it.
+template <typename T> struct Wide {
+    static constexpr int EPQ = 16 / sizeof(T);
+};
+__device__ __forceinline__ float half_bits(uint32_t lo16, float) { return 0.f; }
+__device__ __forceinline__ float half_bits(uint32_t lo16, uint16_t) { return __uint_as_float(lo16 << 16); }
+__device__ __forceinline__ float half_bits(uint32_t lo16, _Float16) { return (float)__builtin_bit_cast(_Float16, (uint16_t)lo16); }
+template <typename T>
+__device__ __forceinline__ void widen(const uint4 &q, float (&x)[Wide<T>::EPQ])
 {
-    if (VEC) {
-        if (c < E) {
-            const typename Quad<T>::type q = *reinterpret_cast<const typename Quad<T>::type *>(row + c);
-            x[0] = widen(q.x, T()); x[1] = widen(q.y, T()); x[2] = widen(q.z, T()); x[3] = widen(q.w, T());
-        } else {
-            x[0] = x[1] = x[2] = x[3] = -INFINITY;
-        }
-    } else {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = c + i < E ? Ld<T>::get(row + c + i) : -INFINITY;
+    for (int i = 0; i < 4; ++i) {
+        if (sizeof(T) == 4) {
+            x[i] = __uint_as_float(w[i]);
+        } else {
+            x[(2 * i) % Wide<T>::EPQ] = half_bits(w[i] & 0xffffu, T());
+            x[(2 * i + 1) % Wide<T>::EPQ] = half_bits(w[i] >> 16, T());
+        }
     }
 }
+template <typename T> struct Lowest;                           // -inf in every element
+template <> struct Lowest<float> { static constexpr uint32_t WORD = 0xff800000u; };
+template <> struct Lowest<uint16_t> { static constexpr uint32_t WORD = 0xff80ff80u; };
+template <> struct Lowest<_Float16> { static constexpr uint32_t WORD = 0xfc00fc00u; };
+
+// a quad from column c; columns at and after E read as -inf.  VEC: rows start on 16 bytes and E is a whole number of quads
 template <typename T, bool VEC>
-__device__ __forceinline__ void store4(T *row, int c, int E, const float (&x)[4])
+__device__ __forceinline__ uint4 load_quad(const T *row, int c, int E)
 {
+    constexpr uint32_t low = Lowest<T>::WORD;
+    if (VEC) return c < E ? *reinterpret_cast<const uint4 *>(row + c) : make_uint4(low, low, low, low);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (sizeof(T) == 4) {
+            w[i] = c + i < E ? reinterpret_cast<const uint32_t *>(row)[c + i] : low;
+        } else {
+            const uint16_t *h = reinterpret_cast<const uint16_t *>(row);
+            const uint32_t lo = c + 2 * i < E ? h[c + 2 * i] : low & 0xffffu, hi = c + 2 * i + 1 < E ? h[c + 2 * i + 1] : low & 0xffffu;
+            w[i] = lo | hi << 16;
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_quad(T *row, int c, int E, const float (&x)[Wide<T>::EPQ])
+{
+    constexpr int EPQ = Wide<T>::EPQ;
     if (VEC) {
         if (c < E) {
-            T q[4];
+            alignas(16) T q[EPQ];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) Ld<T>::put(q + i, x[i]);
-            *reinterpret_cast<typename Quad<T>::type *>(row + c) = *reinterpret_cast<const typename Quad<T>::type *>(q);
+            for (int i = 0; i < EPQ; ++i) Ld<T>::put(q + i, x[i]);
+            *reinterpret_cast<uint4 *>(row + c) = *reinterpret_cast<const uint4 *>(q);
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < EPQ; ++i)
             if (c + i < E) Ld<T>::put(row + c + i, x[i]);
     }
 }
@@ -94,81 +116,121 @@ template <int TL> __device__ __forceinline__ float team_sum(float v)
     return v;
 }
 
-template <typename T, int TL, int NJ, int W, bool VEC>
+// The rows of a team, two of them in flight.  x0: the present row's quads, none: it is padded (its quads hold nothing then)
+template <typename T, int TL, int NQ, int W, bool VEC>
+struct Rows {
+    const T *z;
+    int64_t ld, N, n, step;
+    const uint8_t *padded;
+    int E, t;
+    uint4 x0[NQ], x1[NQ], x2[NQ];
+    bool none, none1, none2;
+
+    __device__ __forceinline__ bool skip(int64_t r) const { return r >= N || (padded && padded[r]); }
+    __device__ __forceinline__ void fetch(int64_t r, bool absent, uint4 (&x)[NQ]) const
+    {
+        if (absent) return;
+        const T *row = z + r * ld;
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) x[j] = load_quad<T, VEC>(row, (j * TL * W + t) * Wide<T>::EPQ, E);
+    }
+    __device__ __forceinline__ void begin()
+    {
+        none = skip(n);
+        none1 = skip(n + step);
+        none2 = skip(n + 2 * step);
+        fetch(n, none, x0);
+        fetch(n + step, none1, x1);
+    }
+    __device__ __forceinline__ bool ahead()                     // issues the row after next; whether the one after that is padded
+    {
+        fetch(n + 2 * step, none2, x2);
+        return skip(n + 3 * step);
+    }
+    __device__ __forceinline__ void advance(bool later)
+    {
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+            x0[j] = x1[j];
+            x1[j] = x2[j];
+        }
+        none = none1;
+        none1 = none2;
+        none2 = later;
+        n += step;
+    }
+};
+
+template <typename T, int TL, int NQ, int W, bool VEC>
 __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_fwd_kernel(const T *__restrict__ z, int64_t ld, const uint8_t *__restrict__ padded,
                                                                           int64_t N, int E, float2 *__restrict__ stats, float *__restrict__ part)
 {
-    constexpr int TEAMS = W > 1 ? 1 : 256 / TL;                 // rows a block works on at a time
-    constexpr int SPAN = TL * W * 4;
+    constexpr int TEAMS = W > 1 ? 1 : 256 / TL, EPQ = Wide<T>::EPQ;
     __shared__ float2 ex[2][W];
     extern __shared__ float cols[];                             // W == 1: the block's column sums
-    const int t = W > 1 ? threadIdx.x : threadIdx.x % TL;
-    const int64_t first = (int64_t)blockIdx.x * TEAMS + (W > 1 ? 0 : threadIdx.x / TL), step = (int64_t)gridDim.x * TEAMS;
-    float acc[NJ][4] = {}, x[NJ][4], y[NJ][4];
-    const auto fetch = [&](int64_t n, float (&v)[NJ][4]) {
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) load4<T, VEC>(z + n * ld, j * SPAN + t * 4, E, v[j]);
-    };
-    const auto next = [&](int64_t n) {                          // the row at or after n that is not padded
-        if (padded)
-            while (n < N && padded[n]) n += step;
-        return n;
-    };
-    int64_t n = next(first);
-    if (n < N) fetch(n, x);
+    Rows<T, TL, NQ, W, VEC> a;
+    a.z = z; a.ld = ld; a.N = N; a.padded = padded; a.E = E;
+    a.t = W > 1 ? threadIdx.x : threadIdx.x % TL;
+    a.n = (int64_t)blockIdx.x * TEAMS + (W > 1 ? 0 : threadIdx.x / TL);
+    a.step = (int64_t)gridDim.x * TEAMS;
+    float acc[NQ][EPQ] = {};
+    a.begin();
     int parity = 0;
-    while (n < N) {
-        const int64_t after = next(n + step);
-        if (after < N) fetch(after, y);
-        float m = -INFINITY, s = 0.f;
+    // the trip count is one for the whole block (a team beyond the last row finds its rows absent), so lanes of a wave stay together
+    for (int64_t left = N - (int64_t)blockIdx.x * TEAMS; left > 0; left -= a.step) {
+        const bool later = a.ahead();
+        if (TL < 64 || !a.none) {                               // teams of one wave run side by side; a wave or block of its own skips
+            float e[NQ][EPQ], m = -INFINITY, s = 0.f;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+            for (int j = 0; j < NQ; ++j) {
+                widen<T>(a.x0[j], e[j]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) m = fmaxf(m, x[j][i]);
-        m = team_max<TL>(m);
-        const float m0 = m == -INFINITY ? 0.f : m;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[j][i] = __expf(x[j][i] - m0);
-                s += x[j][i];
+                for (int i = 0; i < EPQ; ++i) {
+                    if (TL < 64) e[j][i] = a.none ? -INFINITY : e[j][i];
+                    m = fmaxf(m, e[j][i]);
+                }
             }
-        s = team_sum<TL>(s);
-        float M = m, S = s;
-        if (W > 1) {
-            if ((threadIdx.x & 63) == 0) ex[parity][threadIdx.x >> 6] = make_float2(m, s);
-            __syncthreads();
-            M = -INFINITY;
-            S = 0.f;
+            m = team_max<TL>(m);
+            const float m0 = m == -INFINITY ? 0.f : m;
 #pragma unroll
-            for (int w = 0; w < W; ++w) M = fmaxf(M, ex[parity][w].x);
+            for (int j = 0; j < NQ; ++j)
 #pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const float2 o = ex[parity][w];
-                S += o.y == 0.f ? 0.f : o.y * __expf(o.x - M);
+                for (int i = 0; i < EPQ; ++i) {
+                    e[j][i] = __expf(e[j][i] - m0);
+                    s += e[j][i];
+                }
+            s = team_sum<TL>(s);
+            float M = m, S = s;
+            if (W > 1) {
+                if ((threadIdx.x & 63) == 0) ex[parity][threadIdx.x >> 6] = make_float2(m, s);
+                __syncthreads();
+                M = -INFINITY;
+                S = 0.f;
+#pragma unroll
+                for (int w = 0; w < W; ++w) M = fmaxf(M, ex[parity][w].x);
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const float2 o = ex[parity][w];
+                    S += o.y == 0.f ? 0.f : o.y * __expf(o.x - M);
+                }
+                parity ^= 1;
             }
-            parity ^= 1;
+            const float f = s == 0.f ? 0.f : W > 1 ? __expf(m - M) / S : 1.0f / s;
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                for (int i = 0; i < EPQ; ++i) acc[j][i] = fmaf(e[j][i], f, acc[j][i]);
+            if (a.t == 0 && !a.none) stats[a.n] = stats_of(M, S);
         }
-        const float f = W > 1 ? (s == 0.f ? 0.f : __expf(m - M) / S) : (s == 0.f ? 0.f : 1.0f / s);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[j][i] = fmaf(x[j][i], f, acc[j][i]);
-        if (t == 0) stats[n] = stats_of(M, S);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[j][i] = y[j][i];
-        n = after;
+        a.advance(later);
     }
     float *out = part + (int64_t)blockIdx.x * E;
     if (W > 1) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+        for (int j = 0; j < NQ; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int c = j * SPAN + t * 4 + i;
+            for (int i = 0; i < EPQ; ++i) {
+                const int c = (j * TL * W + a.t) * EPQ + i;
                 if (c < E) out[c] = acc[j][i];
             }
         return;
@@ -177,15 +239,15 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_fwd_kernel(const
 #pragma unroll
         for (int o = 32; o >= TL; o >>= 1)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[0][i] += __shfl_xor(acc[0][i], o, 64);
+            for (int i = 0; i < EPQ; ++i) acc[0][i] += __shfl_xor(acc[0][i], o, 64);
     }
     for (int w = 0; w < 4; ++w) {                               // then the waves, one after the other
         if ((int)(threadIdx.x >> 6) == w && (threadIdx.x & 63) < TL) {
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
+            for (int j = 0; j < NQ; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int c = j * SPAN + t * 4 + i;
+                for (int i = 0; i < EPQ; ++i) {
+                    const int c = (j * TL + a.t) * EPQ + i;
                     if (c < E) cols[c] = w ? cols[c] + acc[j][i] : acc[j][i];
                 }
         }
@@ -194,48 +256,47 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_fwd_kernel(const
     for (int c = threadIdx.x; c < E; c += 256) out[c] = cols[c];
 }
 
-template <typename T, int TL, int NJ, int W, bool VEC>
+template <typename T, int TL, int NQ, int W, bool VEC>
 __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_grad_kernel(const T *__restrict__ z, int64_t ld, const uint8_t *__restrict__ padded,
                                                                            int64_t N, int E, const float2 *__restrict__ stats,
                                                                            const float *__restrict__ f, const float *__restrict__ sums,
                                                                            const float *__restrict__ gout, T *__restrict__ dz)
 {
-    constexpr int TEAMS = W > 1 ? 1 : 256 / TL;
-    constexpr int SPAN = TL * W * 4;
+    constexpr int TEAMS = W > 1 ? 1 : 256 / TL, EPQ = Wide<T>::EPQ;
     __shared__ float ex[2][W];
-    const int t = W > 1 ? threadIdx.x : threadIdx.x % TL;
-    const int64_t step = (int64_t)gridDim.x * TEAMS;
-    int64_t n = (int64_t)blockIdx.x * TEAMS + (W > 1 ? 0 : threadIdx.x / TL);
-    float fr[NJ][4], x[NJ][4], y[NJ][4];
+    Rows<T, TL, NQ, W, VEC> a;
+    a.z = z; a.ld = ld; a.N = N; a.padded = padded; a.E = E;
+    a.t = W > 1 ? threadIdx.x : threadIdx.x % TL;
+    a.n = (int64_t)blockIdx.x * TEAMS + (W > 1 ? 0 : threadIdx.x / TL);
+    a.step = (int64_t)gridDim.x * TEAMS;
+    float fr[NQ][EPQ];
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
+    for (int j = 0; j < NQ; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int c = j * SPAN + t * 4 + i;
+        for (int i = 0; i < EPQ; ++i) {
+            const int c = (j * TL * W + a.t) * EPQ + i;
             fr[j][i] = c < E ? f[c] : 0.f;
         }
     const float scale = gout[0] * ((float)E / sums[2 * (int64_t)E]);
-    const auto fetch = [&](int64_t r, float (&v)[NJ][4]) {
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) load4<T, VEC>(z + r * ld, j * SPAN + t * 4, E, v[j]);
-    };
-    const auto skipped = [&](int64_t r) { return padded && padded[r]; };
-    if (n < N && !skipped(n)) fetch(n, x);
+    a.begin();
+    const auto stat = [&](int64_t r, bool absent) { return absent ? make_float2(0.f, 0.f) : stats[r]; };
+    float2 st = stat(a.n, a.none), st1 = stat(a.n + a.step, a.none1);
     int parity = 0;
-    for (; n < N; n += step) {
-        const int64_t after = n + step;
-        if (after < N && !skipped(after)) fetch(after, y);
-        const bool none = skipped(n);
-        const float2 st = none ? make_float2(0.f, 0.f) : stats[n];
-        if (!none) {
+    for (int64_t left = N - (int64_t)blockIdx.x * TEAMS; left > 0; left -= a.step) {
+        const bool later = a.ahead();
+        const float2 st2 = stat(a.n + 2 * a.step, a.none2);
+        float e[NQ][EPQ];
+        if (TL < 64 || !a.none) {
             float s = 0.f;
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
+            for (int j = 0; j < NQ; ++j) {
+                widen<T>(a.x0[j], e[j]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[j][i] = __expf(x[j][i] - st.x) * st.y;
-                    s = fmaf(fr[j][i], x[j][i], s);
+                for (int i = 0; i < EPQ; ++i) {
+                    e[j][i] = __expf(e[j][i] - st.x) * st.y;
+                    s = fmaf(fr[j][i], e[j][i], s);
                 }
+            }
             s = team_sum<TL>(s);
             if (W > 1) {
                 if ((threadIdx.x & 63) == 0) ex[parity][threadIdx.x >> 6] = s;
@@ -246,21 +307,23 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_grad_kernel(cons
                 parity ^= 1;
             }
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
+            for (int j = 0; j < NQ; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[j][i] = scale * x[j][i] * (fr[j][i] - s);
-        } else {
-#pragma unroll
-            for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[j][i] = 0.f;
+                for (int i = 0; i < EPQ; ++i) e[j][i] = scale * e[j][i] * (fr[j][i] - s);
         }
+        if (a.none) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) store4<T, VEC>(dz + n * E, j * SPAN + t * 4, E, x[j]);
+            for (int j = 0; j < NQ; ++j)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+                for (int i = 0; i < EPQ; ++i) e[j][i] = 0.f;
+        }
+        if (a.n < N) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[j][i] = y[j][i];
+            for (int j = 0; j < NQ; ++j) store_quad<T, VEC>(dz + a.n * E, (j * TL * W + a.t) * EPQ, E, e[j]);
+        }
+        a.advance(later);
+        st = st1;
+        st1 = st2;
     }
 }
 
@@ -319,45 +382,61 @@ __global__ __launch_bounds__(256) void balance_cols_kernel(const T *__restrict__
 }
 
 // sums = {sum_n p_ne (E), counts (E), valid rows}: what data-parallel ranks add up before the loss is formed.  A block owns 32 columns: it adds
-// their partial sums (eight threads a column, in f64, joined in order) and reads all assignments for the ones that fall on them, which
-// costs 4 K / 32 bytes out of the L2 per score read and spares a zeroed histogram and its atomics.
+// their partial sums (32 threads a column, in f64, joined in order) and reads all assignments for the ones that fall on them, four to a
+// load: 4 K / 32 bytes out of the L2 per score read, and no histogram in memory that somebody has to clear.
 constexpr int BL_COLS = 32;
+typedef int int4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef long long2u __attribute__((ext_vector_type(2), aligned(8)));
 template <typename I>
-__global__ __launch_bounds__(256) void balance_sums_kernel(const float *__restrict__ part, int nparts, const I *__restrict__ idx,
-                                                           const uint8_t *__restrict__ padded, int64_t N, int K, int E, int32_t *__restrict__ counts,
-                                                           float *__restrict__ sums)
+__global__ __launch_bounds__(1024) void balance_sums_kernel(const float *__restrict__ part, int nparts, const I *__restrict__ idx,
+                                                            const uint8_t *__restrict__ padded, int N, int K, int E, int32_t *__restrict__ counts,
+                                                            float *__restrict__ sums)
 {
-    __shared__ double red[8][BL_COLS];
+    __shared__ double red[32][BL_COLS + 1];
     __shared__ int hist[BL_COLS + 1];
     const int e0 = blockIdx.x * BL_COLS, c = threadIdx.x % BL_COLS, g = threadIdx.x / BL_COLS;
     if (threadIdx.x <= BL_COLS) hist[threadIdx.x] = 0;
     double a = 0.0;
-    if (e0 + c < E)
-        for (int i = g; i < nparts; i += 8) a += (double)part[(int64_t)i * E + e0 + c];
+    if (e0 + c < E) {
+#pragma unroll 4
+        for (int i = g; i < nparts; i += 32) a += (double)part[(int64_t)i * E + e0 + c];
+    }
     red[g][c] = a;
     __syncthreads();
-    int valid = 0;
-    for (int64_t n = threadIdx.x; n < N; n += 256) {
-        if (padded && padded[n]) continue;
-        ++valid;
-        for (int k = 0; k < K; ++k) {
-            const int64_t e = (int64_t)idx[n * K + k] - e0;
-            if (e >= 0 && e < BL_COLS && e + e0 < E) atomicAdd(&hist[e], 1);
+    const int total = N * K, last = min(e0 + BL_COLS, E);
+    const auto count = [&](int i, int64_t e) {
+        if (e < e0 || e >= last) return;
+        if (padded && padded[K == 1 ? i : i / K]) return;
+        atomicAdd(&hist[(int)e - e0], 1);
+    };
+#pragma unroll 4
+    for (int i = threadIdx.x * 4; i < total - 3; i += 4096) {
+        if (sizeof(I) == 4) {
+            const int4u q = *reinterpret_cast<const int4u *>(idx + i);
+            count(i, q.x); count(i + 1, q.y); count(i + 2, q.z); count(i + 3, q.w);
+        } else {
+            const long2u q = *reinterpret_cast<const long2u *>(idx + i), r = *reinterpret_cast<const long2u *>(idx + i + 2);
+            count(i, q.x); count(i + 1, q.y); count(i + 2, r.x); count(i + 3, r.y);
         }
     }
-    if (blockIdx.x == 0) atomicAdd(&hist[BL_COLS], valid);
+    if (threadIdx.x < (total & 3)) count((total & ~3) + threadIdx.x, idx[(total & ~3) + threadIdx.x]);
+    if (blockIdx.x == 0) {
+        int valid = 0;
+        if (padded)
+            for (int n = threadIdx.x; n < N; n += 1024) valid += padded[n] == 0;
+        else if (threadIdx.x == 0)
+            valid = N;
+        atomicAdd(&hist[BL_COLS], valid);
+    }
     __syncthreads();
     if (g == 0 && e0 + c < E) {
         double t = 0.0;
-        for (int i = 0; i < 8; ++i) t += red[i][c];
+        for (int i = 0; i < 32; ++i) t += red[i][c];
         sums[e0 + c] = (float)t;
         sums[E + e0 + c] = (float)hist[c];
         counts[e0 + c] = hist[c];
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-        sums[2 * (int64_t)E] = (float)hist[BL_COLS];
-        counts[E] = hist[BL_COLS];
-    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) sums[2 * (int64_t)E] = (float)hist[BL_COLS];
 }
 
 __global__ __launch_bounds__(1024) void balance_final_kernel(const float *__restrict__ sums, int E, int K, float *__restrict__ loss, float *__restrict__ f)
@@ -407,14 +486,14 @@ __global__ __launch_bounds__(256) void balance_bwd_kernel(const T *__restrict__ 
 
 inline int64_t bl_chunks(int64_t n) { return n < 512 ? n : 512; }
 
-// How a row is held: the smallest team whose lanes hold it in at most 8 quads each.  wide: the kernels above
+// How a row is held: the smallest team that holds it in at most 4 quads a lane.  wide: the two-pass kernels above
 struct BlForm {
-    int tl, nj, w;
+    int tl, nq, w;
     bool wide;
 };
-inline BlForm bl_form(int E)
+inline BlForm bl_form(int E, int dtype)
 {
-    const int q = (E + 3) / 4;                                  // quads of a row
+    const int epq = dtype == 0 ? 4 : 8, q = (E + epq - 1) / epq;   // quads of a row
     if (q <= 4) return {4, 1, 1, false};
     if (q <= 8) return {8, 1, 1, false};
     if (q <= 16) return {16, 1, 1, false};
@@ -422,7 +501,7 @@ inline BlForm bl_form(int E)
     if (q <= 64) return {64, 1, 1, false};
     if (q <= 128) return {64, 2, 1, false};
     if (q <= 256) return {64, 4, 1, false};
-    if (q <= 512) return {64, 8, 1, false};
+    if (q <= 512) return {64, 2, 4, false};
     if (q <= 1024) return {64, 4, 4, false};
     if (q <= 2048) return {64, 4, 8, false};
     if (q <= 4096) return {64, 4, 16, false};
@@ -430,9 +509,9 @@ inline BlForm bl_form(int E)
 }
 inline int bl_blocks(const BlForm &f, int64_t rows)
 {
-    const int64_t teams = f.w > 1 ? 1 : 256 / f.tl, most = f.w > 1 ? 256 * (16 / f.w) : 512;
+    const int64_t teams = f.w > 1 ? 1 : 256 / f.tl;
     const int64_t b = cdiv(rows, teams);
-    return (int)(b < most ? b : most);
+    return (int)(b < 512 ? b : 512);
 }
 
 }  // namespace mq
@@ -440,10 +519,10 @@ inline int bl_blocks(const BlForm &f, int64_t rows)
 using namespace mq;
 
 // partial column sums
-extern "C" size_t mq_code_balance_workspace(int64_t rows, int codes)
+extern "C" size_t mq_code_balance_workspace(int64_t rows, int codes, int dtype)
 {
-    if (rows <= 0 || codes <= 0) return 0;
-    const BlForm f = bl_form(codes);
+    if (rows <= 0 || codes <= 0 || dtype < 0 || dtype > 2) return 0;
+    const BlForm f = bl_form(codes, dtype);
     return (size_t)(f.wide ? bl_chunks(rows) : bl_blocks(f, rows)) * codes * sizeof(float);
 }
 
@@ -453,7 +532,7 @@ extern "C" size_t mq_code_balance_workspace(int64_t rows, int codes)
     case 1: call(uint16_t); break;                                        \
     default: call(_Float16); break;                                       \
     }
-// F(TL, NJ, W): one of the forms of bl_form
+// F(TL, NQ, W): one of the forms of bl_form
 #define BL_FORMS(F)                                                       \
     if (f.tl == 4) F(4, 1, 1);                                            \
     else if (f.tl == 8) F(8, 1, 1);                                       \
@@ -461,21 +540,22 @@ extern "C" size_t mq_code_balance_workspace(int64_t rows, int codes)
     else if (f.tl == 32) F(32, 1, 1);                                     \
     else if (f.w == 16) F(64, 4, 16);                                     \
     else if (f.w == 8) F(64, 4, 8);                                       \
-    else if (f.w == 4) F(64, 4, 4);                                       \
-    else if (f.nj == 1) F(64, 1, 1);                                      \
-    else if (f.nj == 2) F(64, 2, 1);                                      \
-    else if (f.nj == 4) F(64, 4, 1);                                      \
-    else F(64, 8, 1);
+    else if (f.w == 4 && f.nq == 4) F(64, 4, 4);                          \
+    else if (f.w == 4) F(64, 2, 4);                                       \
+    else if (f.nq == 1) F(64, 1, 1);                                      \
+    else if (f.nq == 2) F(64, 2, 1);                                      \
+    else F(64, 4, 1);
 
 template <typename T>
 static void bl_forward(const T *z, int64_t ld, const uint8_t *padded, int64_t rows, int codes, float2 *st, float *part, const BlForm &f, int blocks, hipStream_t s)
 {
-    const bool vec = codes % 4 == 0 && ld % 4 == 0 && (uintptr_t)z % (4 * sizeof(T)) == 0;
-#define F(TL, NJ, W)                                                                                                                                  \
+    const int epq = Wide<T>::EPQ;
+    const bool vec = codes % epq == 0 && ld % epq == 0 && (uintptr_t)z % 16 == 0;
+#define F(TL, NQ, W)                                                                                                                                  \
     do {                                                                                                                                              \
         const size_t lds = W > 1 ? 0 : (size_t)codes * sizeof(float);                                                                                 \
-        if (vec) hipLaunchKernelGGL((balance_fwd_kernel<T, TL, NJ, W, true>), dim3(blocks), dim3(W > 1 ? 64 * W : 256), lds, s, z, ld, padded, rows, codes, st, part); \
-        else hipLaunchKernelGGL((balance_fwd_kernel<T, TL, NJ, W, false>), dim3(blocks), dim3(W > 1 ? 64 * W : 256), lds, s, z, ld, padded, rows, codes, st, part);    \
+        if (vec) hipLaunchKernelGGL((balance_fwd_kernel<T, TL, NQ, W, true>), dim3(blocks), dim3(W > 1 ? 64 * W : 256), lds, s, z, ld, padded, rows, codes, st, part); \
+        else hipLaunchKernelGGL((balance_fwd_kernel<T, TL, NQ, W, false>), dim3(blocks), dim3(W > 1 ? 64 * W : 256), lds, s, z, ld, padded, rows, codes, st, part);    \
     } while (0)
     BL_FORMS(F)
 #undef F
@@ -484,32 +564,33 @@ template <typename T>
 static void bl_backward(const T *z, int64_t ld, const uint8_t *padded, int64_t rows, int codes, const float2 *st, const float *fr, const float *sums, const float *gout, T *dz,
                         const BlForm &f, hipStream_t s)
 {
-    const bool vec = codes % 4 == 0 && ld % 4 == 0 && ((uintptr_t)z | (uintptr_t)dz) % (4 * sizeof(T)) == 0;
+    const int epq = Wide<T>::EPQ;
+    const bool vec = codes % epq == 0 && ld % epq == 0 && ((uintptr_t)z | (uintptr_t)dz) % 16 == 0;
     const int64_t teams = f.w > 1 ? 1 : 256 / f.tl, want = cdiv(rows, teams), most = f.w > 1 ? 256 * (32 / f.w) : 2048;
     const dim3 grid((unsigned)(want < most ? want : most));
-#define F(TL, NJ, W)                                                                                                                                  \
+#define F(TL, NQ, W)                                                                                                                                  \
     do {                                                                                                                                              \
-        if (vec) hipLaunchKernelGGL((balance_grad_kernel<T, TL, NJ, W, true>), grid, dim3(W > 1 ? 64 * W : 256), 0, s, z, ld, padded, rows, codes, st, fr, sums, gout, dz); \
-        else hipLaunchKernelGGL((balance_grad_kernel<T, TL, NJ, W, false>), grid, dim3(W > 1 ? 64 * W : 256), 0, s, z, ld, padded, rows, codes, st, fr, sums, gout, dz);    \
+        if (vec) hipLaunchKernelGGL((balance_grad_kernel<T, TL, NQ, W, true>), grid, dim3(W > 1 ? 64 * W : 256), 0, s, z, ld, padded, rows, codes, st, fr, sums, gout, dz); \
+        else hipLaunchKernelGGL((balance_grad_kernel<T, TL, NQ, W, false>), grid, dim3(W > 1 ? 64 * W : 256), 0, s, z, ld, padded, rows, codes, st, fr, sums, gout, dz);    \
     } while (0)
     BL_FORMS(F)
 #undef F
 }
 
-extern "C" int mq_code_balance_sums(const void *logits, int dtype, int64_t row_stride, const void *idx, int idx64, int per_row, const uint8_t *padded,
-                                    int64_t rows, int codes, void *stats, int32_t *counts, float *sums, void *workspace, size_t workspace_bytes,
-                                    mqStream stream)
+extern "C" int mq_code_balance_fwd(const void *logits, int dtype, int64_t row_stride, const void *idx, int idx64, int per_row, const uint8_t *padded,
+                                    int64_t rows, int codes, void *stats, int32_t *counts, float *sums, float *loss, float *fractions,
+                                    void *workspace, size_t workspace_bytes, mqStream stream)
 {
-    MQ_REQUIRE(logits && idx && stats && counts && sums && workspace, "mq_code_balance_sums: NULL argument");
-    MQ_REQUIRE(dtype >= 0 && dtype <= 2, "mq_code_balance_sums: dtype %d (0 f32, 1 bf16, 2 f16)", dtype);
+    MQ_REQUIRE(logits && idx && stats && counts && sums && workspace && !loss == !fractions, "mq_code_balance_fwd: NULL argument");
+    MQ_REQUIRE(dtype >= 0 && dtype <= 2, "mq_code_balance_fwd: dtype %d (0 f32, 1 bf16, 2 f16)", dtype);
     MQ_REQUIRE(rows > 0 && rows < INT32_MAX && codes > 0 && codes <= (1 << 24) && per_row > 0 && row_stride >= codes,
-               "mq_code_balance_sums: bad sizes (rows %lld, codes %d, per_row %d, row stride %lld)", (long long)rows, codes, per_row, (long long)row_stride);
-    MQ_REQUIRE(rows * (int64_t)per_row < INT32_MAX, "mq_code_balance_sums: the counts would pass 32 bits");
-    MQ_REQUIRE(workspace_bytes >= mq_code_balance_workspace(rows, codes), "mq_code_balance_sums: workspace of %zu bytes, %zu needed", workspace_bytes,
-               mq_code_balance_workspace(rows, codes));
+               "mq_code_balance_fwd: bad sizes (rows %lld, codes %d, per_row %d, row stride %lld)", (long long)rows, codes, per_row, (long long)row_stride);
+    MQ_REQUIRE(rows * (int64_t)per_row <= (1 << 30), "mq_code_balance_fwd: more than 2^30 assignments: the counts would near 32 bits");
+    MQ_REQUIRE(workspace_bytes >= mq_code_balance_workspace(rows, codes, dtype), "mq_code_balance_fwd: workspace of %zu bytes, %zu needed", workspace_bytes,
+               mq_code_balance_workspace(rows, codes, dtype));
     float *part = reinterpret_cast<float *>(workspace);
     float2 *st = reinterpret_cast<float2 *>(stats);
-    const BlForm f = bl_form(codes);
+    const BlForm f = bl_form(codes, dtype);
     int nparts;
     if (f.wide) {
         const int64_t chunk = cdiv(rows, bl_chunks(rows));
@@ -528,10 +609,11 @@ extern "C" int mq_code_balance_sums(const void *logits, int dtype, int64_t row_s
     }
     const dim3 grid((unsigned)cdiv(codes, BL_COLS));
     if (idx64)
-        hipLaunchKernelGGL(balance_sums_kernel<int64_t>, grid, dim3(256), 0, S(stream), part, nparts, reinterpret_cast<const int64_t *>(idx), padded, rows, per_row, codes, counts, sums);
+        hipLaunchKernelGGL(balance_sums_kernel<int64_t>, grid, dim3(1024), 0, S(stream), part, nparts, reinterpret_cast<const int64_t *>(idx), padded, (int)rows, per_row, codes, counts, sums);
     else
-        hipLaunchKernelGGL(balance_sums_kernel<int32_t>, grid, dim3(256), 0, S(stream), part, nparts, reinterpret_cast<const int32_t *>(idx), padded, rows, per_row, codes, counts, sums);
-    MQ_LAUNCH_CHECK("mq_code_balance_sums");
+        hipLaunchKernelGGL(balance_sums_kernel<int32_t>, grid, dim3(1024), 0, S(stream), part, nparts, reinterpret_cast<const int32_t *>(idx), padded, (int)rows, per_row, codes, counts, sums);
+    if (loss) hipLaunchKernelGGL(balance_final_kernel, dim3(1), dim3(1024), 0, S(stream), sums, codes, per_row, loss, fractions);
+    MQ_LAUNCH_CHECK("mq_code_balance_fwd");
     return 0;
 }
 
@@ -550,7 +632,7 @@ extern "C" int mq_code_balance_bwd(const void *logits, int dtype, int64_t row_st
     MQ_REQUIRE(dtype >= 0 && dtype <= 2, "mq_code_balance_bwd: dtype %d (0 f32, 1 bf16, 2 f16)", dtype);
     MQ_REQUIRE(rows > 0 && rows < INT32_MAX && codes > 0 && row_stride >= codes, "mq_code_balance_bwd: bad sizes");
     const float2 *st = reinterpret_cast<const float2 *>(stats);
-    const BlForm form = bl_form(codes);
+    const BlForm form = bl_form(codes, dtype);
     if (form.wide) {
 #define CALL(T)                                                                                                                                       \
     hipLaunchKernelGGL(balance_bwd_kernel<T>, dim3((unsigned)rows), dim3(256), 0, S(stream), reinterpret_cast<const T *>(logits), row_stride, padded, codes, st, fractions, \

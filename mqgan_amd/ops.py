@@ -1603,7 +1603,9 @@ def _score_rows(logits: torch.Tensor, what: str):
     if V == 0:
         raise _lib.MqganHipError(f"{what}: no codes")
     rows = logits.numel() // V
-    z = logits.detach()
+    z = logits
+    if z.is_contiguous():
+        return z, kind, rows, V, V
     stride, ok = V, z.stride(-1) == 1 or V == 1
     dims = [(n, s) for n, s in zip(z.shape[:-1], z.stride()[:-1]) if n != 1]
     if dims:
@@ -1627,7 +1629,7 @@ def _row_mask(padded, rows, like, what):
         return None
     if padded.dtype not in (torch.uint8, torch.bool) or padded.numel() != rows:
         raise _lib.MqganHipError(f"{what}: padded is uint8 or bool with one value per row ({rows}), got {padded.dtype} {tuple(padded.shape)}")
-    return padded.reshape(-1).to(torch.uint8).contiguous()
+    return padded.contiguous()                      # a bool is a byte of 0 or 1
 
 
 def sample_codes(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, padded=None, return_logp=False):
@@ -1660,54 +1662,63 @@ def sample_codes(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, t
         d = _lib.SampleDesc(rows, stride, V, kind, 0.0 if t is not None else float(temperature), 0.0 if p is not None else float(top_p),
                             0.0 if m is not None else float(min_p), 0 if k is not None else min(int(top_k), V))
         check(L().mq_sample_codes(C.byref(d), _score_ptr(z), fptr(u), fptr(t, True), ptr(k, torch.int32, True), fptr(p, True), fptr(m, True),
-                                  ptr(mask, torch.uint8, True), ptr(idx, torch.int64), fptr(logp, True), stream()), "mq_sample_codes")
+                                  ptr(mask, None, True), ptr(idx, torch.int64), fptr(logp, True), stream()), "mq_sample_codes")
     return (idx, logp) if return_logp else idx
 
 
 class CodeBalanceFn(torch.autograd.Function):
-    """(loss, counts) of losses.code_balance_loss."""
+    """(loss, counts) of losses.code_balance_loss.  One scratch tensor holds the rows' statistics, the sums, the fractions and the partial sums."""
 
     @staticmethod
     def forward(ctx, logits, idx, padded, comm):
         z, kind, rows, V, stride = _score_rows(logits, "code_balance_loss")
         K = idx.shape[-1] if idx.dim() == logits.dim() else 1
-        if idx.dtype not in (torch.int32, torch.int64) or tuple(idx.shape) not in (tuple(logits.shape[:-1]), tuple(logits.shape[:-1]) + (K,)):
-            raise _lib.MqganHipError(f"code_balance_loss: int32 / int64 codes of shape {tuple(logits.shape[:-1])} or with the assignments of a row "
-                                     f"behind, got {idx.dtype} {tuple(idx.shape)}")
+        lead = logits.shape[:-1]
+        if idx.dtype not in (torch.int32, torch.int64) or (idx.shape != lead and idx.shape != lead + (K,)):
+            raise _lib.MqganHipError(f"code_balance_loss: int32 / int64 codes of shape {tuple(lead)} or with the assignments of a row behind, got "
+                                     f"{idx.dtype} {tuple(idx.shape)}")
+        if K == 0:
+            raise _lib.MqganHipError("code_balance_loss: no assignments")
         mask = _row_mask(padded, rows, z, "code_balance_loss")
-        sums = _empty((2 * V + 1,), z)
-        counts = torch.empty((V + 1,), dtype=torch.int32, device=z.device)
-        stats = _empty((max(rows, 1), 2), z)
-        idx = idx.contiguous()
-        if rows and K:
-            nbytes = L().mq_code_balance_workspace(rows, V)
-            ws = _ws_bytes(nbytes, z)
-            check(L().mq_code_balance_sums(_score_ptr(z), kind, stride, ptr(idx), int(idx.dtype == torch.int64), K, ptr(mask, torch.uint8, True),
-                                           rows, V, ptr(stats), ptr(counts), fptr(sums), ptr(ws), ws.numel(), stream()), "mq_code_balance_sums")
+        lib = L()
+        n_stats, n_sums = 2 * rows + (rows & 1) * 2, (2 * V + 4) // 4 * 4
+        nbytes = lib.mq_code_balance_workspace(rows, V, kind)
+        scratch = _empty((n_stats + n_sums + V + 3 + nbytes // 4,), z)
+        counts = torch.empty((V,), dtype=torch.int32, device=z.device)
+        loss = _empty((), z)
+        zp, at = _score_ptr(z), fptr(scratch).value
+        sums, f, ws = at + 4 * n_stats, at + 4 * (n_stats + n_sums), at + 4 * (n_stats + n_sums + (V + 3) // 4 * 4)
+        together = comm is not None and comm.active
+        if rows:
+            idx = idx.contiguous()
+            check(lib.mq_code_balance_fwd(zp, kind, stride, ptr(idx), int(idx.dtype == torch.int64), K, ptr(mask, None, True), rows, V, at,
+                                          ptr(counts), sums, None if together else fptr(loss), None if together else f, ws, nbytes, stream()),
+                  "mq_code_balance_fwd")
         else:
-            sums.zero_()
+            scratch.zero_()
             counts.zero_()
-        if comm is not None and comm.active:
-            _reduce(comm, sums)
-            counts = sums[V:].to(torch.int32)
-        loss, f = _empty((1,), z), _empty((V,), z)
-        check(L().mq_code_balance_final(fptr(sums), V, max(K, 1), fptr(loss), fptr(f), stream()), "mq_code_balance_final")
-        ctx.save_for_backward(z, mask, stats, sums, f)
-        ctx.cfg = (kind, rows, V, stride, logits.shape)
-        counts = counts[:V]
+        if together or not rows:
+            if together:
+                s = scratch[n_stats:n_stats + 2 * V + 1]
+                _reduce(comm, s)
+                counts = s[V:2 * V].to(torch.int32)
+            check(lib.mq_code_balance_final(sums, V, K, fptr(loss), f, stream()), "mq_code_balance_final")
+        ctx.save_for_backward(z, mask, scratch)
+        ctx.cfg = (kind, rows, V, stride, logits.shape, sums - at, f - at)
         ctx.mark_non_differentiable(counts)
-        return loss.view(()), counts
+        return loss, counts
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gout, _):
-        z, mask, stats, sums, f = ctx.saved_tensors
-        kind, rows, V, stride, shape = ctx.cfg
+        z, mask, scratch = ctx.saved_tensors
+        kind, rows, V, stride, shape, sums, f = ctx.cfg
+        if torch.is_grad_enabled():
+            raise _lib.MqganHipError("code_balance_loss: its gradient cannot be differentiated again (create_graph)")
         dz = torch.empty(shape, dtype=z.dtype, device=z.device)
         if rows:
-            g = gout.to(F32).contiguous().view(1)
-            check(L().mq_code_balance_bwd(_score_ptr(z), kind, stride, ptr(mask, torch.uint8, True), rows, V, ptr(stats), fptr(sums), fptr(f),
-                                          fptr(g), ptr(dz), stream()), "mq_code_balance_bwd")
+            at = scratch.data_ptr()
+            check(L().mq_code_balance_bwd(_score_ptr(z), kind, stride, ptr(mask, None, True), rows, V, at, at + sums, at + f, fptr(gout), ptr(dz),
+                                          stream()), "mq_code_balance_bwd")
         return dz, None, None, None
 
 

@@ -74,9 +74,10 @@ def test_step_follows_the_formula(grad, unaligned, max_norm, grad_scale):
             ev = t * 7 * H32 * (old_v + v64 + (1 - b2) * (g64 * coef) ** 2)
             _near(m_all[at:at + p.numel()], m64, em + 1e-44, f"step {t} tensor {i} exp_avg")
             _near(v_all[at:at + p.numel()], v64, ev + 1e-44, f"step {t} tensor {i} exp_avg_sq")
-            # the update: m's and half of v's error, and eight roundings (both factors, root, product, sum, quotient, product); p: two a step
+            # the update: m's and half of v's error, six roundings (both factors, product, sum, two products), and one ulp - two half steps -
+            # each of the root and the reciprocal; p: two roundings a step
             upd = rate / (1 - b1 ** t) * m64.abs() / (torch.sqrt(v64 / (1 - b2 ** t)) + eps)
-            e_upd = rate / (1 - b1 ** t) * em / (torch.sqrt(v64 / (1 - b2 ** t)) + eps) + upd * (ev / v64.clamp(min=1e-60) + 9 * H32)
+            e_upd = rate / (1 - b1 ** t) * em / (torch.sqrt(v64 / (1 - b2 ** t)) + eps) + upd * (ev / v64.clamp(min=1e-60) + 10 * H32)
             _near(p, p64, 3 * H32 * (old_p.abs() + p64.abs() + upd) + e_upd, f"step {t} tensor {i} parameter")
             ref[i] = (p.double().cpu(), m_all[at:at + p.numel()].double().cpu(), v_all[at:at + p.numel()].double().cpu())
     for buf, p, o in leaves:                          # the neighbours of every parameter stay as they were

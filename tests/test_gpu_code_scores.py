@@ -434,12 +434,21 @@ def test_balance_is_the_same_on_every_run_and_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(out, want)), r
 
 
+def test_balance_gradient_is_not_differentiated_again():
+    from mqgan_amd._lib import MqganHipError
+    from mqgan_amd.losses import code_balance_loss
+    z = torch.randn(4, 10, device=DEV, requires_grad=True)
+    loss, _ = code_balance_loss(z, torch.zeros(4, dtype=torch.int32, device=DEV))
+    with pytest.raises(MqganHipError, match="again"):
+        torch.autograd.grad(loss, z, create_graph=True)
+
+
 def test_balance_refusals():
     from mqgan_amd._lib import MqganHipError
     from mqgan_amd.losses import code_balance_loss
     z, i = torch.zeros(4, 10, device=DEV), torch.zeros(4, dtype=torch.int32, device=DEV)
     for bad in (lambda: code_balance_loss(z.double(), i), lambda: code_balance_loss(z, i[:3]), lambda: code_balance_loss(z, i.float()),
                 lambda: code_balance_loss(z, i, torch.zeros(4, device=DEV)), lambda: code_balance_loss(z, i, torch.zeros(3, dtype=torch.uint8, device=DEV)),
-                lambda: code_balance_loss(z.cpu(), i), lambda: code_balance_loss(z, i.cpu()), lambda: code_balance_loss(z[:, :0], i)):
+                lambda: code_balance_loss(z, i[:, None][:, :0]), lambda: code_balance_loss(z.cpu(), i), lambda: code_balance_loss(z, i.cpu()), lambda: code_balance_loss(z[:, :0], i)):
         with pytest.raises(MqganHipError):
             bad()

@@ -45,16 +45,16 @@ def test_sample_codes_refuses_on_the_host(lib):
 
 
 def test_code_balance_refuses_on_the_host(lib):
-    def sums(z=A, dtype=0, ld=10, idx=A, K=1, rows=4, codes=10, stats=A, counts=A, out=A, ws=A, n=1 << 20):
-        return lib.mq_code_balance_sums(z, dtype, ld, idx, 0, K, None, rows, codes, stats, counts, out, ws, n, None)
-    for a in ("z", "idx", "stats", "counts", "out", "ws"):
+    def sums(z=A, dtype=0, ld=10, idx=A, K=1, rows=4, codes=10, stats=A, counts=A, out=A, loss=A, f=A, ws=A, n=1 << 20):
+        return lib.mq_code_balance_fwd(z, dtype, ld, idx, 0, K, None, rows, codes, stats, counts, out, loss, f, ws, n, None)
+    for a in ("z", "idx", "stats", "counts", "out", "ws", "loss", "f"):
         refused(lib, sums(**{a: None}), b"NULL")
     refused(lib, sums(dtype=3), b"dtype")
     for kw in ({"rows": 0}, {"rows": 2 ** 31}, {"codes": 0}, {"codes": (1 << 24) + 1, "ld": 1 << 25}, {"K": 0}, {"ld": 9}):
         refused(lib, sums(**kw), b"bad sizes")
     refused(lib, sums(rows=2 ** 30, K=4), b"32 bits")
-    need = lib.mq_code_balance_workspace(4, 10)
-    assert need > 0 and lib.mq_code_balance_workspace(0, 10) == 0 and lib.mq_code_balance_workspace(4, 0) == 0
+    need = lib.mq_code_balance_workspace(4, 10, 0)
+    assert need > 0 and lib.mq_code_balance_workspace(0, 10, 0) == 0 and lib.mq_code_balance_workspace(4, 0, 0) == 0 and lib.mq_code_balance_workspace(4, 10, 3) == 0
     refused(lib, sums(n=need - 1), b"workspace")
     refused(lib, lib.mq_code_balance_final(A, 0, 1, A, A, None), b"bad arguments")
     refused(lib, lib.mq_code_balance_final(None, 4, 1, A, A, None), b"bad arguments")
