@@ -5,8 +5,10 @@
 // E codes, K assignments a row, Nv rows that are not padded.  L is 1 where codes are used evenly and E where one code takes all.  The
 // counts are whole numbers and carry no gradient.
 //
-// A row's statistics are its maximum m and 1 / sum exp(z - m), never their logarithm's sum: a row of nothing but the type's lowest value
-// has log(sum) far under half an ulp of m.  A row of -inf alone has p = 0.  Padded rows are not read; their gradient is 0.
+// A row's statistics are an offset and a factor, p = factor * 2^(z log2 e - offset), and never one logarithm for both: a row of nothing but the
+// type's lowest value has log(sum) far under half an ulp of its maximum.  The offset is the maximum times log2 e, rounded; all of a row
+// uses the same, so its rounding goes into the factor.  Where that product could overflow (|maximum| > 1e37) the maximum itself is kept, as
+// a difference first: Offset.  A row of -inf alone has p = 0.  Padded rows are not read; their gradient is 0.
 #include "common.h"
 
 namespace mq {
@@ -29,17 +31,49 @@ template <> struct Ld<_Float16> {
     static __device__ __forceinline__ void put(_Float16 *p, float v) { *p = (_Float16)v; }
 };
 
-__device__ __forceinline__ float2 stats_of(float m, float s)            // (subtrahend, factor) of a row
+constexpr float LOG2E = 1.44269504088896340736f;
+struct Offset {
+    float o;                             // max log2 e, or the maximum itself where it is huge
+    bool huge;
+    __device__ __forceinline__ explicit Offset(float m) : o(m == -INFINITY ? 0.f : m), huge(fabsf(o) > 1e37f) { o = huge ? o : o * LOG2E; }
+    __device__ __forceinline__ Offset(float2 stats) : o(stats.x), huge(stats.y < 0.f) {}
+    __device__ __forceinline__ float exp(float z) const { return __builtin_amdgcn_exp2f(huge ? (z - o) * LOG2E : fmaf(z, LOG2E, -o)); }
+};
+// what a sum over part of a row, whose maximum is m, counts for in the row's, whose maximum is M
+__device__ __forceinline__ float rebase(float m, float M)
 {
-    return m == -INFINITY ? make_float2(0.f, s) : make_float2(m, 1.0f / s);      // s is 0 here, or a NaN
+    const Offset a(m), b(M);
+    return __builtin_amdgcn_exp2f(a.huge || b.huge ? (m - M) * LOG2E : a.o - b.o);
+}
+// (offset, factor); the factor is negative where the offset is the maximum itself
+__device__ __forceinline__ float2 stats_of(float m, float s)
+{
+    const Offset a(m);
+    const float f = m == -INFINITY ? s : 1.0f / s;              // s is 0 in a row of -inf alone, or a NaN
+    return make_float2(a.o, a.huge ? -f : f);
+}
+// x <- 2^(x log2 e - offset); the two ways as a branch, which all lanes of a wave nearly always take together
+template <int NQ, int EPQ>
+__device__ __forceinline__ void exp_all(float (&x)[NQ][EPQ], const Offset &f)
+{
+    if (__builtin_amdgcn_ballot_w64(f.huge) == 0) {
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+            for (int i = 0; i < EPQ; ++i) x[j][i] = __builtin_amdgcn_exp2f(fmaf(x[j][i], LOG2E, -f.o));
+    } else {
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+            for (int i = 0; i < EPQ; ++i) x[j][i] = f.exp(x[j][i]);
+    }
 }
 
 // ----------------------------------------------------------------------------- a row in registers, read once
 // A team of TL lanes (a part of a wave), or of W whole waves (then TL = 64), holds one row as NQ quads of 16 bytes a lane: lane t the
 // columns (j TL W + t) EPQ .. + EPQ - 1, j < NQ.  The columns of a lane are the same for every row, so the sums over rows are registers too
 // and the row's own maximum and sum are the only things that cross lanes (shuffles; with W > 1 one LDS exchange and one barrier a row,
-// the buffer alternating).  Two rows are in flight behind the one that is worked on, as they lie in memory (bf16 takes half the registers);
-// what says whether a row is padded is read one row further ahead, so that no load waits for it.
+// the buffer alternating).  Two rows are in flight behind the one that is worked on, as they lie in memory (bf16 takes half the registers).
 template <typename T> struct Wide {
     static constexpr int EPQ = 16 / sizeof(T);
 };
@@ -66,11 +100,17 @@ template <> struct Lowest<uint16_t> { static constexpr uint32_t WORD = 0xff80ff8
 template <> struct Lowest<_Float16> { static constexpr uint32_t WORD = 0xfc00fc00u; };
 
 // a quad from column c; columns at and after E read as -inf.  VEC: rows start on 16 bytes and E is a whole number of quads
-template <typename T, bool VEC>
+// NT: a non-temporal load.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+template <typename T, bool VEC, bool NT>
 __device__ __forceinline__ uint4 load_quad(const T *row, int c, int E)
 {
     constexpr uint32_t low = Lowest<T>::WORD;
-    if (VEC) return c < E ? *reinterpret_cast<const uint4 *>(row + c) : make_uint4(low, low, low, low);
+    if (VEC) {
+        u32x4 q = {low, low, low, low};
+        if (c < E) q = NT ? __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(row + c)) : *reinterpret_cast<const u32x4 *>(row + c);
+        return make_uint4(q.x, q.y, q.z, q.w);
+    }
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -93,7 +133,7 @@ __device__ __forceinline__ void store_quad(T *row, int c, int E, const float (&x
             alignas(16) T q[EPQ];
 #pragma unroll
             for (int i = 0; i < EPQ; ++i) Ld<T>::put(q + i, x[i]);
-            *reinterpret_cast<uint4 *>(row + c) = *reinterpret_cast<const uint4 *>(q);
+            __builtin_nontemporal_store(*reinterpret_cast<const u32x4 *>(q), reinterpret_cast<u32x4 *>(row + c));
         }
     } else {
 #pragma unroll
@@ -116,8 +156,24 @@ template <int TL> __device__ __forceinline__ float team_sum(float v)
     return v;
 }
 
+// over the 16 lanes of a DPP row, in every lane of it
+__device__ __forceinline__ float row16_max(float v)
+{
+    v = fmaxf(v, dpp_mov<0xB1>(v, v));
+    v = fmaxf(v, dpp_mov<0x4E>(v, v));
+    v = fmaxf(v, dpp_mov<0x141>(v, v));
+    return fmaxf(v, dpp_mov<0x140>(v, v));
+}
+__device__ __forceinline__ float row16_sum(float v)
+{
+    v += dpp_mov<0xB1>(0.f, v);
+    v += dpp_mov<0x4E>(0.f, v);
+    v += dpp_mov<0x141>(0.f, v);
+    return v + dpp_mov<0x140>(0.f, v);
+}
+
 // The rows of a team, two of them in flight.  x0: the present row's quads, none: it is padded (its quads hold nothing then)
-template <typename T, int TL, int NQ, int W, bool VEC>
+template <typename T, int TL, int NQ, int W, bool VEC, bool NT>
 struct Rows {
     const T *z;
     int64_t ld, N, n, step;
@@ -125,29 +181,33 @@ struct Rows {
     int E, t;
     uint4 x0[NQ], x1[NQ], x2[NQ];
     bool none, none1, none2;
+    uint32_t pad3, pad4;                                        // the flags of the rows three and four on, as loaded: compared when their turn comes
 
-    __device__ __forceinline__ bool skip(int64_t r) const { return r >= N || (padded && padded[r]); }
+    __device__ __forceinline__ uint32_t flag(int64_t r) const { return r >= N ? 1u : padded ? (uint32_t)padded[r] : 0u; }
     __device__ __forceinline__ void fetch(int64_t r, bool absent, uint4 (&x)[NQ]) const
     {
         if (absent) return;
         const T *row = z + r * ld;
 #pragma unroll
-        for (int j = 0; j < NQ; ++j) x[j] = load_quad<T, VEC>(row, (j * TL * W + t) * Wide<T>::EPQ, E);
+        for (int j = 0; j < NQ; ++j) x[j] = load_quad<T, VEC, NT>(row, (j * TL * W + t) * Wide<T>::EPQ, E);
     }
     __device__ __forceinline__ void begin()
     {
-        none = skip(n);
-        none1 = skip(n + step);
-        none2 = skip(n + 2 * step);
+        none = flag(n) != 0;
+        none1 = flag(n + step) != 0;
+        none2 = flag(n + 2 * step) != 0;
+        pad3 = flag(n + 3 * step);
         fetch(n, none, x0);
         fetch(n + step, none1, x1);
     }
-    __device__ __forceinline__ bool ahead()                     // issues the row after next; whether the one after that is padded
+    // Issues the row after next, and before it the flag of the row four on: loads return in order, a flag behind the row's quads would be
+    // waited for together with them.
+    __device__ __forceinline__ void ahead()
     {
+        pad4 = flag(n + 4 * step);
         fetch(n + 2 * step, none2, x2);
-        return skip(n + 3 * step);
     }
-    __device__ __forceinline__ void advance(bool later)
+    __device__ __forceinline__ void advance()
     {
 #pragma unroll
         for (int j = 0; j < NQ; ++j) {
@@ -156,19 +216,45 @@ struct Rows {
         }
         none = none1;
         none1 = none2;
-        none2 = later;
+        none2 = pad3 != 0;
+        pad3 = pad4;
         n += step;
     }
 };
 
+// The assignments as the kernels take them: int32, or int64 with wide = 1
+struct Codes {
+    const void *p;
+    int wide, K;
+    __device__ __forceinline__ int64_t at(int64_t i) const { return wide ? reinterpret_cast<const int64_t *>(p)[i] : (int64_t) reinterpret_cast<const int32_t *>(p)[i]; }
+};
+
+// Besides its rows a block of W == 1 counts a slice of the assignments (and of the valid rows) in LDS: pcount (blocks, E + 1).
 template <typename T, int TL, int NQ, int W, bool VEC>
 __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_fwd_kernel(const T *__restrict__ z, int64_t ld, const uint8_t *__restrict__ padded,
-                                                                          int64_t N, int E, float2 *__restrict__ stats, float *__restrict__ part)
+                                                                          int64_t N, int E, float2 *__restrict__ stats, float *__restrict__ part,
+                                                                          const Codes codes, int32_t *__restrict__ pcount)
 {
     constexpr int TEAMS = W > 1 ? 1 : 256 / TL, EPQ = Wide<T>::EPQ;
     __shared__ float2 ex[2][W];
-    extern __shared__ float cols[];                             // W == 1: the block's column sums
-    Rows<T, TL, NQ, W, VEC> a;
+    extern __shared__ float cols[];                             // W == 1: the block's counts, then its column sums
+    if (W == 1) {
+        int *hist = reinterpret_cast<int *>(cols);
+        for (int c = threadIdx.x; c <= E; c += 256) hist[c] = 0;
+        __syncthreads();
+        const int64_t per = (N + gridDim.x - 1) / gridDim.x, r0 = blockIdx.x * per, r1 = r0 + per < N ? r0 + per : N;
+        for (int64_t i = r0 * codes.K + threadIdx.x; i < r1 * codes.K; i += 256) {
+            const int64_t r = codes.K == 1 ? i : i / codes.K, c = codes.at(i);
+            if (padded && padded[r]) continue;
+            if (c >= 0 && c < E) atomicAdd(hist + c, 1);
+            if (i == r * codes.K) atomicAdd(hist + E, 1);
+        }
+        __syncthreads();
+        int32_t *to = pcount + (int64_t)blockIdx.x * (E + 1);
+        for (int c = threadIdx.x; c <= E; c += 256) to[c] = hist[c];
+        __syncthreads();
+    }
+    Rows<T, TL, NQ, W, VEC, false> a;
     a.z = z; a.ld = ld; a.N = N; a.padded = padded; a.E = E;
     a.t = W > 1 ? threadIdx.x : threadIdx.x % TL;
     a.n = (int64_t)blockIdx.x * TEAMS + (W > 1 ? 0 : threadIdx.x / TL);
@@ -178,7 +264,7 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_fwd_kernel(const
     int parity = 0;
     // the trip count is one for the whole block (a team beyond the last row finds its rows absent), so lanes of a wave stay together
     for (int64_t left = N - (int64_t)blockIdx.x * TEAMS; left > 0; left -= a.step) {
-        const bool later = a.ahead();
+        a.ahead();
         if (TL < 64 || !a.none) {                               // teams of one wave run side by side; a wave or block of its own skips
             float e[NQ][EPQ], m = -INFINITY, s = 0.f;
 #pragma unroll
@@ -191,38 +277,30 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_fwd_kernel(const
                 }
             }
             m = team_max<TL>(m);
-            const float m0 = m == -INFINITY ? 0.f : m;
+            exp_all(e, Offset(m));
 #pragma unroll
             for (int j = 0; j < NQ; ++j)
 #pragma unroll
-                for (int i = 0; i < EPQ; ++i) {
-                    e[j][i] = __expf(e[j][i] - m0);
-                    s += e[j][i];
-                }
+                for (int i = 0; i < EPQ; ++i) s += e[j][i];
             s = team_sum<TL>(s);
             float M = m, S = s;
             if (W > 1) {
                 if ((threadIdx.x & 63) == 0) ex[parity][threadIdx.x >> 6] = make_float2(m, s);
                 __syncthreads();
-                M = -INFINITY;
-                S = 0.f;
-#pragma unroll
-                for (int w = 0; w < W; ++w) M = fmaxf(M, ex[parity][w].x);
-#pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    const float2 o = ex[parity][w];
-                    S += o.y == 0.f ? 0.f : o.y * __expf(o.x - M);
-                }
+                const int w = threadIdx.x & 15;                 // a lane a wave's pair; W <= 16
+                const float2 o = w < W ? ex[parity][w] : make_float2(-INFINITY, 0.f);
+                M = row16_max(o.x);
+                S = row16_sum(o.y == 0.f ? 0.f : o.y * rebase(o.x, M));
                 parity ^= 1;
             }
-            const float f = s == 0.f ? 0.f : W > 1 ? __expf(m - M) / S : 1.0f / s;
+            const float f = s == 0.f ? 0.f : W > 1 ? rebase(m, M) / S : 1.0f / s;
 #pragma unroll
             for (int j = 0; j < NQ; ++j)
 #pragma unroll
                 for (int i = 0; i < EPQ; ++i) acc[j][i] = fmaf(e[j][i], f, acc[j][i]);
             if (a.t == 0 && !a.none) stats[a.n] = stats_of(M, S);
         }
-        a.advance(later);
+        a.advance();
     }
     float *out = part + (int64_t)blockIdx.x * E;
     if (W > 1) {
@@ -264,7 +342,7 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_grad_kernel(cons
 {
     constexpr int TEAMS = W > 1 ? 1 : 256 / TL, EPQ = Wide<T>::EPQ;
     __shared__ float ex[2][W];
-    Rows<T, TL, NQ, W, VEC> a;
+    Rows<T, TL, NQ, W, VEC, true> a;
     a.z = z; a.ld = ld; a.N = N; a.padded = padded; a.E = E;
     a.t = W > 1 ? threadIdx.x : threadIdx.x % TL;
     a.n = (int64_t)blockIdx.x * TEAMS + (W > 1 ? 0 : threadIdx.x / TL);
@@ -283,7 +361,7 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_grad_kernel(cons
     float2 st = stat(a.n, a.none), st1 = stat(a.n + a.step, a.none1);
     int parity = 0;
     for (int64_t left = N - (int64_t)blockIdx.x * TEAMS; left > 0; left -= a.step) {
-        const bool later = a.ahead();
+        a.ahead();
         const float2 st2 = stat(a.n + 2 * a.step, a.none2);
         float e[NQ][EPQ];
         if (TL < 64 || !a.none) {
@@ -291,13 +369,13 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_grad_kernel(cons
 #pragma unroll
             for (int j = 0; j < NQ; ++j) {
                 widen<T>(a.x0[j], e[j]);
-#pragma unroll
-                for (int i = 0; i < EPQ; ++i) {
-                    e[j][i] = __expf(e[j][i] - st.x) * st.y;
-                    s = fmaf(fr[j][i], e[j][i], s);
-                }
             }
-            s = team_sum<TL>(s);
+            exp_all(e, Offset(st));
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+#pragma unroll
+                for (int i = 0; i < EPQ; ++i) s = fmaf(fr[j][i], e[j][i], s);
+            s = team_sum<TL>(s) * fabsf(st.y);
             if (W > 1) {
                 if ((threadIdx.x & 63) == 0) ex[parity][threadIdx.x >> 6] = s;
                 __syncthreads();
@@ -306,10 +384,11 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_grad_kernel(cons
                 for (int w = 0; w < W; ++w) s += ex[parity][w];
                 parity ^= 1;
             }
+            const float by = scale * fabsf(st.y);
 #pragma unroll
             for (int j = 0; j < NQ; ++j)
 #pragma unroll
-                for (int i = 0; i < EPQ; ++i) e[j][i] = scale * e[j][i] * (fr[j][i] - s);
+                for (int i = 0; i < EPQ; ++i) e[j][i] = by * e[j][i] * (fr[j][i] - s);
         }
         if (a.none) {
 #pragma unroll
@@ -321,7 +400,7 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_grad_kernel(cons
 #pragma unroll
             for (int j = 0; j < NQ; ++j) store_quad<T, VEC>(dz + a.n * E, (j * TL * W + a.t) * EPQ, E, e[j]);
         }
-        a.advance(later);
+        a.advance();
         st = st1;
         st1 = st2;
     }
@@ -332,7 +411,7 @@ __global__ __launch_bounds__(W > 1 ? 64 * W : 256) void balance_grad_kernel(cons
 __device__ __forceinline__ float2 block_join(float m, float s, float *red)
 {
     const float wm = wave_max(m);
-    const float ws = wave_sum(s == 0.f ? 0.f : s * __expf(m - wm));
+    const float ws = wave_sum(s == 0.f ? 0.f : s * rebase(m, wm));
     __syncthreads();
     if ((threadIdx.x & 63) == 0) {
         red[threadIdx.x >> 6] = wm;
@@ -341,7 +420,7 @@ __device__ __forceinline__ float2 block_join(float m, float s, float *red)
     __syncthreads();
     const float M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     float S = 0.f;
-    for (int i = 0; i < 4; ++i) S += red[4 + i] == 0.f ? 0.f : red[4 + i] * __expf(red[i] - M);
+    for (int i = 0; i < 4; ++i) S += red[4 + i] == 0.f ? 0.f : red[4 + i] * rebase(red[i], M);
     return make_float2(M, S);
 }
 
@@ -357,7 +436,7 @@ __global__ __launch_bounds__(256) void balance_rows_kernel(const T *__restrict__
     for (int e = threadIdx.x; e < E; e += 256) {
         const float x = Ld<T>::get(row + e);
         const float nm = fmaxf(m, x);
-        s = (s == 0.f ? 0.f : s * __expf(m - nm)) + (x == -INFINITY ? 0.f : __expf(x - nm));
+        s = (s == 0.f ? 0.f : s * rebase(m, nm)) + (x == -INFINITY ? 0.f : Offset(nm).exp(x));
         m = nm;
     }
     const float2 j = block_join(m, s, red);
@@ -376,57 +455,63 @@ __global__ __launch_bounds__(256) void balance_cols_kernel(const T *__restrict__
     for (int64_t n = n0; n < n1; ++n) {
         if (padded && padded[n]) continue;
         const float2 st = stats[n];
-        a = fmaf(__expf(Ld<T>::get(z + n * ld + e) - st.x), st.y, a);
+        a = fmaf(Offset(st).exp(Ld<T>::get(z + n * ld + e)), fabsf(st.y), a);
     }
     part[(int64_t)blockIdx.y * E + e] = a;
 }
 
-// sums = {sum_n p_ne (E), counts (E), valid rows}: what data-parallel ranks add up before the loss is formed.  A block owns 32 columns: it adds
-// their partial sums (32 threads a column, in f64, joined in order) and reads all assignments for the ones that fall on them, four to a
-// load: 4 K / 32 bytes out of the L2 per score read, and no histogram in memory that somebody has to clear.
+// sums = {sum_n p_ne (E), counts (E), valid rows}: what data-parallel ranks add up before the loss is formed.  A block owns 32 columns and
+// adds their partial sums (32 threads a column, in f64, joined in order).  The counts come as partial sums too (pcount), or - the forms
+// without a histogram - each block reads all assignments for the ones that fall on its columns, four to a load (4 K / 32 bytes out of the
+// L2 per score read), and one more block counts the valid rows.
 constexpr int BL_COLS = 32;
 typedef int int4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef long long2u __attribute__((ext_vector_type(2), aligned(8)));
-template <typename I>
-__global__ __launch_bounds__(1024) void balance_sums_kernel(const float *__restrict__ part, int nparts, const I *__restrict__ idx,
-                                                            const uint8_t *__restrict__ padded, int N, int K, int E, int32_t *__restrict__ counts,
+__global__ __launch_bounds__(1024) void balance_sums_kernel(const float *__restrict__ part, const int32_t *__restrict__ pcount, int nparts, const Codes codes,
+                                                            const uint8_t *__restrict__ padded, int N, int E, int32_t *__restrict__ counts,
                                                             float *__restrict__ sums)
 {
     __shared__ double red[32][BL_COLS + 1];
-    __shared__ int hist[BL_COLS + 1];
+    __shared__ int hist[BL_COLS];
     const int e0 = blockIdx.x * BL_COLS, c = threadIdx.x % BL_COLS, g = threadIdx.x / BL_COLS;
-    if (threadIdx.x <= BL_COLS) hist[threadIdx.x] = 0;
+    if (threadIdx.x < BL_COLS) hist[threadIdx.x] = 0;
+    __syncthreads();
     double a = 0.0;
     if (e0 + c < E) {
 #pragma unroll 4
         for (int i = g; i < nparts; i += 32) a += (double)part[(int64_t)i * E + e0 + c];
     }
     red[g][c] = a;
-    __syncthreads();
-    const int total = N * K, last = min(e0 + BL_COLS, E);
-    const auto count = [&](int i, int64_t e) {
-        if (e < e0 || e >= last) return;
-        if (padded && padded[K == 1 ? i : i / K]) return;
-        atomicAdd(&hist[(int)e - e0], 1);
-    };
+    if (pcount) {
+        int n = 0;
+        if (e0 + c <= E) {
 #pragma unroll 4
-    for (int i = threadIdx.x * 4; i < total - 3; i += 4096) {
-        if (sizeof(I) == 4) {
-            const int4u q = *reinterpret_cast<const int4u *>(idx + i);
-            count(i, q.x); count(i + 1, q.y); count(i + 2, q.z); count(i + 3, q.w);
-        } else {
-            const long2u q = *reinterpret_cast<const long2u *>(idx + i), r = *reinterpret_cast<const long2u *>(idx + i + 2);
-            count(i, q.x); count(i + 1, q.y); count(i + 2, r.x); count(i + 3, r.y);
+            for (int i = g; i < nparts; i += 32) n += pcount[(int64_t)i * (E + 1) + e0 + c];
         }
-    }
-    if (threadIdx.x < (total & 3)) count((total & ~3) + threadIdx.x, idx[(total & ~3) + threadIdx.x]);
-    if (blockIdx.x == 0) {
-        int valid = 0;
-        if (padded)
-            for (int n = threadIdx.x; n < N; n += 1024) valid += padded[n] == 0;
-        else if (threadIdx.x == 0)
-            valid = N;
-        atomicAdd(&hist[BL_COLS], valid);
+        if (n) atomicAdd(&hist[c], n);
+    } else if (e0 >= E) {                                       // the block behind the columns
+        int n = 0;
+        for (int r = threadIdx.x; r < N; r += 1024) n += !(padded && padded[r]);
+        atomicAdd(&hist[0], n);
+    } else {
+        const int total = N * codes.K, last = min(e0 + BL_COLS, E);
+        const auto count = [&](int i, int64_t e) {
+            if (e < e0 || e >= last) return;
+            if (padded && padded[codes.K == 1 ? i : i / codes.K]) return;
+            atomicAdd(&hist[(int)e - e0], 1);
+        };
+#pragma unroll 4
+        for (int i = threadIdx.x * 4; i < total - 3; i += 4096) {
+            if (codes.wide) {
+                const long *p = reinterpret_cast<const long *>(codes.p) + i;
+                const long2u q = *reinterpret_cast<const long2u *>(p), r = *reinterpret_cast<const long2u *>(p + 2);
+                count(i, q.x); count(i + 1, q.y); count(i + 2, r.x); count(i + 3, r.y);
+            } else {
+                const int4u q = *reinterpret_cast<const int4u *>(reinterpret_cast<const int *>(codes.p) + i);
+                count(i, q.x); count(i + 1, q.y); count(i + 2, q.z); count(i + 3, q.w);
+            }
+        }
+        if (threadIdx.x < (total & 3)) count((total & ~3) + threadIdx.x, codes.at((total & ~3) + threadIdx.x));
     }
     __syncthreads();
     if (g == 0 && e0 + c < E) {
@@ -436,7 +521,7 @@ __global__ __launch_bounds__(1024) void balance_sums_kernel(const float *__restr
         sums[E + e0 + c] = (float)hist[c];
         counts[e0 + c] = hist[c];
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) sums[2 * (int64_t)E] = (float)hist[BL_COLS];
+    if (g == 0 && (pcount ? e0 + c == E : e0 >= E && c == 0)) sums[2 * (int64_t)E] = (float)hist[c];
 }
 
 __global__ __launch_bounds__(1024) void balance_final_kernel(const float *__restrict__ sums, int E, int K, float *__restrict__ loss, float *__restrict__ f)
@@ -475,11 +560,11 @@ __global__ __launch_bounds__(256) void balance_bwd_kernel(const T *__restrict__ 
     const T *row = z + n * ld;
     const float2 st = stats[n];
     float s = 0.f;
-    for (int e = threadIdx.x; e < E; e += 256) s = fmaf(f[e], __expf(Ld<T>::get(row + e) - st.x) * st.y, s);
+    for (int e = threadIdx.x; e < E; e += 256) s = fmaf(f[e], Offset(st).exp(Ld<T>::get(row + e)) * fabsf(st.y), s);
     s = block_sum<256>(s, red);
     const float scale = gout[0] * ((float)E / sums[2 * (int64_t)E]);
     for (int e = threadIdx.x; e < E; e += 256) {
-        const float p = __expf(Ld<T>::get(row + e) - st.x) * st.y;
+        const float p = Offset(st).exp(Ld<T>::get(row + e)) * fabsf(st.y);
         Ld<T>::put(out + e, scale * p * (f[e] - s));
     }
 }
@@ -502,7 +587,7 @@ inline BlForm bl_form(int E, int dtype)
     if (q <= 128) return {64, 2, 1, false};
     if (q <= 256) return {64, 4, 1, false};
     if (q <= 512) return {64, 2, 4, false};
-    if (q <= 1024) return {64, 4, 4, false};
+    if (q <= 1024) return {64, 2, 8, false};
     if (q <= 2048) return {64, 4, 8, false};
     if (q <= 4096) return {64, 4, 16, false};
     return {0, 0, 0, true};
@@ -523,7 +608,7 @@ extern "C" size_t mq_code_balance_workspace(int64_t rows, int codes, int dtype)
 {
     if (rows <= 0 || codes <= 0 || dtype < 0 || dtype > 2) return 0;
     const BlForm f = bl_form(codes, dtype);
-    return (size_t)(f.wide ? bl_chunks(rows) : bl_blocks(f, rows)) * codes * sizeof(float);
+    return f.wide ? (size_t)bl_chunks(rows) * codes * 4 : (size_t)bl_blocks(f, rows) * ((size_t)codes * 4 + (f.w > 1 ? 0 : ((size_t)codes + 1) * 4));
 }
 
 #define BL_TYPES(call)                                                    \
@@ -539,23 +624,24 @@ extern "C" size_t mq_code_balance_workspace(int64_t rows, int codes, int dtype)
     else if (f.tl == 16) F(16, 1, 1);                                     \
     else if (f.tl == 32) F(32, 1, 1);                                     \
     else if (f.w == 16) F(64, 4, 16);                                     \
-    else if (f.w == 8) F(64, 4, 8);                                       \
-    else if (f.w == 4 && f.nq == 4) F(64, 4, 4);                          \
+    else if (f.w == 8 && f.nq == 4) F(64, 4, 8);                          \
+    else if (f.w == 8) F(64, 2, 8);                                       \
     else if (f.w == 4) F(64, 2, 4);                                       \
     else if (f.nq == 1) F(64, 1, 1);                                      \
     else if (f.nq == 2) F(64, 2, 1);                                      \
     else F(64, 4, 1);
 
 template <typename T>
-static void bl_forward(const T *z, int64_t ld, const uint8_t *padded, int64_t rows, int codes, float2 *st, float *part, const BlForm &f, int blocks, hipStream_t s)
+static void bl_forward(const T *z, int64_t ld, const uint8_t *padded, int64_t rows, int codes, float2 *st, float *part, const BlForm &f, int blocks, const Codes &c,
+                       int32_t *pcount, hipStream_t s)
 {
     const int epq = Wide<T>::EPQ;
     const bool vec = codes % epq == 0 && ld % epq == 0 && (uintptr_t)z % 16 == 0;
 #define F(TL, NQ, W)                                                                                                                                  \
     do {                                                                                                                                              \
-        const size_t lds = W > 1 ? 0 : (size_t)codes * sizeof(float);                                                                                 \
-        if (vec) hipLaunchKernelGGL((balance_fwd_kernel<T, TL, NQ, W, true>), dim3(blocks), dim3(W > 1 ? 64 * W : 256), lds, s, z, ld, padded, rows, codes, st, part); \
-        else hipLaunchKernelGGL((balance_fwd_kernel<T, TL, NQ, W, false>), dim3(blocks), dim3(W > 1 ? 64 * W : 256), lds, s, z, ld, padded, rows, codes, st, part);    \
+        const size_t lds = W > 1 ? 0 : ((size_t)codes + 1) * sizeof(float);                                                                                 \
+        if (vec) hipLaunchKernelGGL((balance_fwd_kernel<T, TL, NQ, W, true>), dim3(blocks), dim3(W > 1 ? 64 * W : 256), lds, s, z, ld, padded, rows, codes, st, part, c, pcount); \
+        else hipLaunchKernelGGL((balance_fwd_kernel<T, TL, NQ, W, false>), dim3(blocks), dim3(W > 1 ? 64 * W : 256), lds, s, z, ld, padded, rows, codes, st, part, c, pcount);    \
     } while (0)
     BL_FORMS(F)
 #undef F
@@ -591,6 +677,8 @@ extern "C" int mq_code_balance_fwd(const void *logits, int dtype, int64_t row_st
     float *part = reinterpret_cast<float *>(workspace);
     float2 *st = reinterpret_cast<float2 *>(stats);
     const BlForm f = bl_form(codes, dtype);
+    const Codes c{idx, idx64, per_row};
+    int32_t *pcount = nullptr;
     int nparts;
     if (f.wide) {
         const int64_t chunk = cdiv(rows, bl_chunks(rows));
@@ -603,15 +691,13 @@ extern "C" int mq_code_balance_fwd(const void *logits, int dtype, int64_t row_st
 #undef CALL
     } else {
         nparts = bl_blocks(f, rows);
-#define CALL(T) bl_forward(reinterpret_cast<const T *>(logits), row_stride, padded, rows, codes, st, part, f, nparts, S(stream))
+        if (f.w == 1) pcount = reinterpret_cast<int32_t *>(part + (int64_t)nparts * codes);
+#define CALL(T) bl_forward(reinterpret_cast<const T *>(logits), row_stride, padded, rows, codes, st, part, f, nparts, c, pcount, S(stream))
         BL_TYPES(CALL)
 #undef CALL
     }
-    const dim3 grid((unsigned)cdiv(codes, BL_COLS));
-    if (idx64)
-        hipLaunchKernelGGL(balance_sums_kernel<int64_t>, grid, dim3(1024), 0, S(stream), part, nparts, reinterpret_cast<const int64_t *>(idx), padded, (int)rows, per_row, codes, counts, sums);
-    else
-        hipLaunchKernelGGL(balance_sums_kernel<int32_t>, grid, dim3(1024), 0, S(stream), part, nparts, reinterpret_cast<const int32_t *>(idx), padded, (int)rows, per_row, codes, counts, sums);
+    const unsigned grid = pcount ? (unsigned)cdiv(codes + 1, BL_COLS) : (unsigned)cdiv(codes, BL_COLS) + 1;
+    hipLaunchKernelGGL(balance_sums_kernel, dim3(grid), dim3(1024), 0, S(stream), part, pcount, nparts, c, padded, (int)rows, codes, counts, sums);
     if (loss) hipLaunchKernelGGL(balance_final_kernel, dim3(1), dim3(1024), 0, S(stream), sums, codes, per_row, loss, fractions);
     MQ_LAUNCH_CHECK("mq_code_balance_fwd");
     return 0;
