@@ -589,7 +589,7 @@ inline BlForm bl_form(int E, int dtype)
     if (q <= 512) return {64, 2, 4, false};
     if (q <= 1024) return {64, 2, 8, false};
     if (q <= 2048) return {64, 4, 8, false};
-    if (q <= 4096) return {64, 4, 16, false};
+    if (q <= 4096 && dtype == 0) return {64, 4, 16, false};          // of two-byte scores it would not fit the registers
     return {0, 0, 0, true};
 }
 inline int bl_blocks(const BlForm &f, int64_t rows)

@@ -73,7 +73,7 @@ def check_draws(z, u, **kw):
     assert edge <= max(2, len(rows) // 50), edge
 
 
-SETTINGS = [{}, {"temperature": 0.7}, {"top_k": 1}, {"top_k": 5}, {"top_p": 0.9}, {"min_p": 0.1}, {"top_p": 0.0}, {"temperature": 0.0},
+SETTINGS = [{}, {"temperature": 1e-310}, {"temperature": 0.7}, {"top_k": 1}, {"top_k": 5}, {"top_p": 0.9}, {"min_p": 0.1}, {"top_p": 0.0}, {"temperature": 0.0},
             {"temperature": 1.3, "top_k": 40, "top_p": 0.8, "min_p": 0.02}, {"temperature": 3.0, "top_k": 300, "top_p": 0.999}]
 
 
@@ -124,7 +124,7 @@ def test_draws_with_infinite_and_undefined_scores():
     from mqgan_amd import ops
     z = torch.tensor([[0.0, INF, 1.0, INF], [float("nan"), 1.0, float("nan"), -INF], [float("nan")] * 4, [-INF] * 4, [1.0, 2.0, 3.0, 4.0]], device=DEV)
     u = torch.tensor([0.6, 0.99, 0.5, 0.5, 2.0], device=DEV)
-    for s in SETTINGS[:2]:
+    for s in SETTINGS[:3]:
         idx, logp = ops.sample_codes(z, u, return_logp=True, **s)
         assert idx.tolist() == [3, 1, -1, -1, 3]
         assert logp[:4].tolist() == pytest.approx([math.log(0.5), 0.0, 0.0, 0.0], abs=1e-7)
