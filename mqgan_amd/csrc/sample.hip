@@ -13,11 +13,12 @@
 // the unit counts as one unit (2^-49 at V = 8192) unless exp gives 0.
 //
 // Both cuts are a place in the order, (score, index): everything at or before it stays.  A block has one row; where it fits (48 KiB) the row is
-// read once, into LDS.  A cut is found without sorting: a histogram over the distance from the maximum (bins of equal RATIO, so neither the
-// scores' scale nor masks of the type's lowest value matter) tells the bin that the cut falls into, a second one over that bin's lower bits
-// narrows it, and the few codes left are put into a list and counted against each other.  Where that list overflows (hundreds of equal scores
-// across the cut) radix selection over the bits of the score finds the cut instead.  Once a cut leaves few codes they are put
-// into a list in index order that takes the row's place: after a top-k the f64 exponentials are those of the codes it keeps.
+// read once, into LDS.  Mostly a bound tells that the first cut lies among few codes - k of the threads' own maxima are at least so large; the
+// codes beyond some distance hold less mass than top_p leaves out - and then these become a list, in index order, that one wave works
+// on alone: the blocks' barriers were what the time went into.  A cut is found without sorting: a histogram over the distance from the maximum
+// (bins of equal RATIO, so neither the scores' scale nor masks of the type's lowest value matter) tells the bin that it falls into, a second
+// one over that bin's lower bits narrows it, and the few codes left are put into a list and counted against each other.  Where that list
+// overflows (hundreds of equal scores across the cut) radix selection over the bits of the score finds the cut instead.
 // A wave covers a contiguous part of the row, so that sums up to a code need one number per wave.
 #include "common.h"
 
@@ -120,48 +121,46 @@ struct Row {
     double scale;                        // 2^shift
     double min_p;                        // <= 1
     // Units of a code with a score above -inf: w 2^shift to the nearest whole number, at least 1 - the bits of w 2^shift + 2^52 (shift <= 51,
-    // w <= 1); 0 where w would underflow and, with FILTER, where it is under min_p.
-    template <bool FILTER>
-    __device__ __forceinline__ uint64_t units(float x) const
+    // w <= 1); 0 where w would underflow and where it is under `least`.
+    __device__ __forceinline__ uint64_t units(float x, double least = 0.0) const
     {
         const double d = ((double)x - max) * per_t, w = exp_neg(fmax(d, -746.0));
         const uint64_t q = (uint64_t)__double_as_longlong(fma(w, scale, 4503599627370496.0)) & 0xfffffffffffffull;
-        return d < -745.0 || (FILTER && w < min_p) ? 0 : q > 1 ? q : 1;
+        return d < -745.0 || w < least ? 0 : q > 1 ? q : 1;
     }
     // log of a weight's share of Z units
     __device__ __forceinline__ float logp(float x, uint64_t Z) const { return (float)(((double)x - max) * per_t - log((double)Z / scale)); }
 };
 
-__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v)
+// Inclusive scans over the 64 lanes by DPP (row shifts, then the rows' last lanes broadcast): a tenth of the latency of the LDS crossbar's.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_from(uint32_t v)             // 0 where there is no lane to read
 {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor((unsigned long long)v, o, 64);
-    return v;
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_from(uint64_t v)
+{
+    return (uint64_t)dpp_from<CTRL, ROWS>((uint32_t)v) | (uint64_t)dpp_from<CTRL, ROWS>((uint32_t)(v >> 32)) << 32;
 }
 template <typename U>
-__device__ __forceinline__ U wave_scan(U v)                          // inclusive
+__device__ __forceinline__ U wave_scan(U v)
 {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const U t = __shfl_up(v, o, 64);
-        if (lane >= o) v += t;
-    }
+    v += dpp_from<0x111, 0xf>(v);                                    // row_shr 1, 2, 4, 8
+    v += dpp_from<0x112, 0xf>(v);
+    v += dpp_from<0x114, 0xf>(v);
+    v += dpp_from<0x118, 0xf>(v);
+    v += dpp_from<0x142, 0xa>(v);                                    // row_bcast 15 into rows 1 and 3
+    v += dpp_from<0x143, 0xc>(v);                                    // row_bcast 31 into rows 2 and 3
     return v;
 }
-// over a block of W waves; red: W entries of its own, free again when the call returns
-template <int W>
-__device__ __forceinline__ uint64_t block_sum_u64(uint64_t v, unsigned long long *red)
+__device__ __forceinline__ uint32_t from_lane(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }      // lane: the same in all
+__device__ __forceinline__ uint64_t from_lane(uint64_t v, int lane)
 {
-    v = wave_sum_u64(v);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    uint64_t t = 0;
-#pragma unroll
-    for (int i = 0; i < W; ++i) t += red[i];
-    __syncthreads();
-    return t;
+    return (uint64_t)from_lane((uint32_t)v, lane) | (uint64_t)from_lane((uint32_t)(v >> 32), lane) << 32;
 }
+template <typename U>
+__device__ __forceinline__ U wave_total(U v) { return from_lane(wave_scan(v), 63); }
 template <int W>
 __device__ __forceinline__ float block_max_f32(float v, float *red)
 {
@@ -182,7 +181,8 @@ struct Found {
     unsigned long long before, total;
     int bin;
 };
-template <int BINS, bool FROM_TOP, typename U>
+template <int W> __device__ __forceinline__ void together();
+template <int BINS, bool FROM_TOP, int W, typename U>
 __device__ __forceinline__ void find_bin(const U *hist, uint64_t goal, Found *out)
 {
     if (threadIdx.x < 64) {
@@ -190,7 +190,7 @@ __device__ __forceinline__ void find_bin(const U *hist, uint64_t goal, Found *ou
         uint64_t mine = 0;
 #pragma unroll
         for (int i = 0; i < PER; ++i) mine += hist[FROM_TOP ? BINS - 1 - ((int)threadIdx.x * PER + i) : (int)threadIdx.x * PER + i];
-        const uint64_t upto = wave_scan<unsigned long long>(mine);
+        const uint64_t upto = wave_scan(mine);
         if (threadIdx.x == 63) out->total = upto;
         if (upto >= goal && upto - mine < goal) {
             uint64_t before = upto - mine;
@@ -204,7 +204,7 @@ __device__ __forceinline__ void find_bin(const U *hist, uint64_t goal, Found *ou
             out->bin = FROM_TOP ? BINS - 1 - ((int)threadIdx.x * PER + i) : (int)threadIdx.x * PER + i;
         }
     }
-    __syncthreads();
+    together<W>();
 }
 
 // order-preserving key of a score
@@ -226,6 +226,8 @@ struct Bins {
         const int b = (int)(__float_as_uint(d) >> SH) - ((127 - 12) << (23 - SH));
         return min(max(b, 0), BINS - 1);
     }
+    // the largest distance in bin b (of an inner one)
+    static __device__ __forceinline__ float end(int b) { return __uint_as_float((uint32_t)(b + 1 + ((127 - 12) << (23 - SH))) << SH) * 0.99999994f; }
     static __device__ __forceinline__ int inner(float d) { return (int)(__float_as_uint(d) >> (SH - LOG)) & (BINS - 1); }
 };
 
@@ -239,7 +241,7 @@ struct Entry {
 };
 template <int DT, int W>
 struct Lds {
-    static constexpr int BINS = W <= 2 ? 256 : 512, LIST = BINS / 2, KEPT = BINS;
+    static constexpr int BINS = W <= 2 ? 256 : 512, LIST = BINS / 2, KEPT = W <= 2 ? 256 : W <= 4 ? 512 : 1024;
     unsigned long long hist[BINS];
     Entry list[LIST];                                               // codes of the bin that a cut falls into
     alignas(16) typename Score<DT>::Raw kept_x[KEPT];               // the kept codes in index order, once they are few
@@ -250,33 +252,43 @@ struct Lds {
     Found found;
 };
 
-template <int DT, bool STAGED, int W>
+// W waves of a block work together on a row; with W = 1 one wave works on by itself, the others have left.
+template <int W>
+__device__ __forceinline__ void together()
+{
+    if (W > 1) __syncthreads();
+    else {                                                           // a wave's LDS accesses are carried out in its order
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+}
+// L: the block's LDS (of its own number of waves)
+template <int DT, bool STAGED, int W, typename L>
 struct Draw {
     static constexpr int NT = 64 * W, FEW = 40;
-    typedef Lds<DT, W> L;
     typedef Bins<L::BINS> B;
     L &s;
     View<DT, STAGED> row;
     float cut_x;                                                    // kept: at or before (cut_x, cut_i) in the order
     int cut_i;
 
-    __device__ __forceinline__ Draw(L &s_) : s(s_) {}
+    __device__ __forceinline__ Draw(L &s_, const View<DT, STAGED> &v) : s(s_), row(v), cut_x(-INFINITY), cut_i(-1) {}      // nothing with a score of -inf
     // The wave's part of the row: codes [from, to), a multiple of 256 from the last one's
-    __device__ __forceinline__ int from(int wave) const { return wave * part(); }
+    __device__ __forceinline__ int wave() const { return W > 1 ? (int)(threadIdx.x >> 6) : 0; }
     __device__ __forceinline__ int part() const { return (row.n + 256 * W - 1) / (256 * W) * 256; }
+    __device__ __forceinline__ int from() const { return wave() * part(); }
+    __device__ __forceinline__ int to() const { return min(from() + part(), row.n); }
     __device__ __forceinline__ bool kept(float x, int c) const { return x > cut_x || (x == cut_x && c <= cut_i); }
-    // f(x, c) for the kept codes of the block
+    // f(x, c) for the kept codes, one at a time: a small loop, there are several of them and the instruction cache is shared
     template <typename F>
     __device__ __forceinline__ void each(F f) const
     {
-        const int c0 = from(threadIdx.x >> 6), c1 = min(c0 + part(), row.n);
+        const int c1 = to();
 #pragma unroll 1
-        for (int c = c0 + (threadIdx.x & 63) * 4; c < c1; c += 256) {
-            float x[4];
-            row.four(c, x);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (kept(x[i], c + i)) f(x[i], c + i);
+        for (int c = from() + (threadIdx.x & 63); c < c1; c += 64) {
+            const float x = row.one(c);
+            if (kept(x, c)) f(x, c);
         }
     }
     // Sum of q(x) over the kept codes of the lane, four at a time without branches between them
@@ -284,9 +296,9 @@ struct Draw {
     __device__ __forceinline__ uint64_t sum(Q q) const
     {
         uint64_t t = 0;
-        const int c0 = from(threadIdx.x >> 6), c1 = min(c0 + part(), row.n);
+        const int c1 = to();
 #pragma unroll 1
-        for (int c = c0 + (threadIdx.x & 63) * 4; c < c1; c += 256) {
+        for (int c = from() + (threadIdx.x & 63) * 4; c < c1; c += 256) {
             float x[4];
             row.four(c, x);
             bool in[4], any = false;
@@ -309,15 +321,15 @@ struct Draw {
         uint64_t above = 0;
 #pragma unroll 1
         for (int sh = 24; sh >= 0; sh -= 8) {
-            __syncthreads();
-            for (int b = threadIdx.x; b < 256; b += NT) s.hist[b] = 0;
-            __syncthreads();
+            together<W>();
+            for (int b = (threadIdx.x & (NT - 1)); b < 256; b += NT) s.hist[b] = 0;
+            together<W>();
             each([&](float v, int) {
                 const uint32_t key = key_of(v);
                 if (sh == 24 || key >> (sh + 8) == prefix) atomicAdd(&s.hist[(key >> sh) & 255u], (unsigned long long)q(v));
             });
-            __syncthreads();
-            find_bin<256, true>(s.hist, goal - above, &s.found);
+            together<W>();
+            find_bin<256, true, W>(s.hist, goal - above, &s.found);
             prefix = prefix << 8 | (uint32_t)s.found.bin;
             above += s.found.before;
         }
@@ -325,66 +337,59 @@ struct Draw {
         const float border = score_of(prefix);
         const uint64_t w = q(border);
         const int need = (int)((goal - above + w - 1) / w);
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        const int c0 = from(wave), c1 = min(c0 + part(), row.n);
-        int count = 0;
-        each([&](float v, int) { count += v == border; });
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) count += __shfl_xor(count, o, 64);
-        if (lane == 0) s.redi[wave] = count;
-        __syncthreads();
+        const int lane = threadIdx.x & 63, c0 = from(), c1 = to();
+        uint32_t mine = 0;
+        each([&](float v, int) { mine += v == border; });
+        const int count = (int)wave_total(mine);
+        if (lane == 0) s.redi[wave()] = count;
+        together<W>();
         int before = 0;
-        for (int v = 0; v < wave; ++v) before += s.redi[v];
+        for (int v = 0; v < wave(); ++v) before += s.redi[v];
         if (before < need && before + count >= need) {
 #pragma unroll 1
             for (int c = c0; c < c1; c += 256) {                    // the wave's lanes go round together
                 float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 const int at = c + lane * 4;
                 if (at < c1) row.four(at, x);
-                int mine = 0;
+                uint32_t here = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) mine += x[i] == border && kept(x[i], at + i);
-                int upto = wave_scan(mine) + before;
-                before = __shfl(upto, 63, 64);
-                upto -= mine;
+                for (int i = 0; i < 4; ++i) here += x[i] == border && kept(x[i], at + i);
+                const uint32_t scan = wave_scan(here);
+                int upto = before + (int)(scan - here);
+                before += (int)from_lane(scan, 63);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (x[i] == border && kept(x[i], at + i) && ++upto == need) s.cut_i = at + i;
             }
         }
-        __syncthreads();
+        together<W>();
         cut_x = border;
         cut_i = s.cut_i;
     }
-    // Moves the cut to the code with which the mass of the kept codes, in their order, reaches `goal` (leaves it if it does not).  q(x): a code's
-    // mass.  limit: a bin that the cut is believed not to lie behind; codes behind it take no part (they do if the belief was wrong).
+    // Moves the cut to the code with which the mass of the kept codes, in their order, reaches `goal`.  q(x): a code's mass.  False: they have
+    // less than that, the cut is where it was.
     template <typename Q>
-    __device__ __forceinline__ void find_cut(float mx, uint64_t goal, int limit, Q q)
+    __device__ __forceinline__ bool find_cut(float mx, uint64_t goal, Q q)
     {
-        const int tid = threadIdx.x;
+        const int tid = threadIdx.x & (NT - 1);
         int bin = 0, sub = -1;
         uint64_t above = 0;
 #pragma unroll 1
         for (int level = 0; level < 2; ++level) {
-            __syncthreads();
+            together<W>();
 #pragma unroll 1
             for (int b = tid; b < L::BINS; b += NT) s.hist[b] = 0;
             if (tid == 0) s.length = 0;
-            __syncthreads();
+            together<W>();
             each([&](float v, int) {
                 const float d = mx - v;
                 const int b = B::of(d);
-                if (level == 0 ? b <= limit : b == bin) atomicAdd(&s.hist[level == 0 ? b : B::inner(d)], (unsigned long long)q(v));
+                if (level == 0 || b == bin) atomicAdd(&s.hist[level == 0 ? b : B::inner(d)], (unsigned long long)q(v));
             });
-            __syncthreads();
-            find_bin<L::BINS, false>(s.hist, goal - above, &s.found);
+            together<W>();
+            find_bin<L::BINS, false, W>(s.hist, goal - above, &s.found);
             if (level == 0) {
-                if (s.found.total < goal) {
-                    if (limit == L::BINS - 1) return;
-                    limit = L::BINS - 1;
-                    level = -1;
-                    continue;
-                }
+                if (s.found.total < goal) return false;
                 bin = s.found.bin;
             } else {
                 sub = s.found.bin;
@@ -396,13 +401,13 @@ struct Draw {
                 const int e = atomicAdd(&s.length, 1);
                 if (e < L::LIST) s.list[e] = Entry{v, c, (unsigned long long)q(v)};
             });
-            __syncthreads();
+            together<W>();
             if (s.length <= FEW || bin == 0 || bin == L::BINS - 1) break;
         }
         const int many = s.length;
         if (many > L::LIST) {
             find_cut_by_bits(goal, q);
-            return;
+            return true;
         }
 #pragma unroll 1
         for (int e = tid; e < many; e += NT) {
@@ -418,85 +423,165 @@ struct Draw {
                 s.cut_i = me.i;
             }
         }
-        __syncthreads();
+        together<W>();
         cut_x = s.cut_x;
         cut_i = s.cut_i;
+        return true;
     }
-    // A bin that at least `goal` codes lie up to: the one that `goal` of the threads' own maxima do.  One number a thread instead of its codes.
-    __device__ __forceinline__ int limit_of(float mx, float own, int goal)
+    // The cuts among the row's codes, and the draw.  Z: the mass of all codes if it is known (they may be more than this row's), else 0.
+    template <typename A>
+    __device__ __forceinline__ void finish(const Row &r, float mx, int k, double P, float u, uint64_t Z, A answer)
     {
-        if (goal > NT) return L::BINS - 1;
-        for (int b = threadIdx.x; b < L::BINS; b += NT) s.hist[b] = 0;
-        __syncthreads();
-        if (own > -INFINITY) atomicAdd(&s.hist[B::of(mx - own)], 1ull);
-        __syncthreads();
-        find_bin<L::BINS, false>(s.hist, (uint64_t)goal, &s.found);
-        return s.found.total < (uint64_t)goal ? L::BINS - 1 : s.found.bin;
+        const int lane = threadIdx.x & 63;
+#pragma unroll 1
+        for (int stage = 0; stage < 2; ++stage) {                   // one copy of find_cut for both: the code has to stay in the instruction cache
+            uint64_t goal = (uint64_t)k;
+            if (stage == 0) {
+                if (k <= 0) continue;
+            } else {
+                if (!(P < 1.0)) continue;
+                if (!Z) Z = total(sum([&](float v) { return r.units(v); }));
+                goal = goal_of(P, Z);
+            }
+            find_cut(mx, goal, [&](float v) { return stage == 0 ? (uint64_t)1 : r.units(v); });
+        }
+        // the waves' sums, then the wave that the draw falls to goes over its part again (NaN min_p: nothing is under it)
+        const uint64_t part_ = wave_total(sum([&](float v) { return r.units(v, r.min_p); }));
+        together<W>();
+        if (lane == 0) s.red[wave()] = part_;
+        together<W>();
+        uint64_t mass = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) mass += s.red[w];
+        const double t = floor((double)(u > 0.f ? u : 0.f) * (double)mass);
+        uint64_t target = t < (double)mass ? (uint64_t)t : mass - 1;
+        if (target >= mass) target = mass - 1;
+        uint64_t before = 0;
+        int mine = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const uint64_t here = s.red[w];
+            if (before + here <= target) {
+                before += here;
+                mine = w + 1;
+            } else {
+                break;
+            }
+        }
+        if (wave() != mine) return;
+        const int c1 = to();
+#pragma unroll 1
+        for (int c = from(); c < c1; c += 256) {                    // the wave's lanes go round together
+            float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            const int at = c + lane * 4;
+            if (at < c1) row.four(at, x);
+            uint64_t q[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[i] = kept(x[i], at + i) ? r.units(x[i], r.min_p) : 0;
+            const uint64_t four = (q[0] + q[1]) + (q[2] + q[3]), upto = wave_scan(four) + before;
+            if (upto > target && upto - four <= target) {
+                uint64_t b = upto - four;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (b <= target && b + q[i] > target) answer(at + i, x[i], mass);
+                    b += q[i];
+                }
+            }
+            before = from_lane(upto, 63);
+            if (before > target) return;
+        }
     }
-    // Where at most KEPT codes are kept: they take the row's place (a row in LDS only), in index order.  Whether they did.
-    __device__ __forceinline__ bool compact()
+    // over the waves
+    __device__ __forceinline__ uint64_t total(uint64_t v) const
     {
-        if (!STAGED) return false;
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        v = wave_total(v);
+        if (W == 1) return v;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) s.red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        uint64_t t = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) t += s.red[w];
+        return t;
+    }
+    // codes are kept while less than this lies before them
+    static __device__ __forceinline__ uint64_t goal_of(double P, uint64_t Z)
+    {
+        const double g = ceil(P * (double)Z);
+        return g > 1.0 ? (uint64_t)g : 1;
+    }
+    // Puts the codes with x >= floor into the list of kept codes, in index order, where they are at most KEPT.  How many they are.
+    __device__ __forceinline__ int compact(float floor)
+    {
+        const int lane = threadIdx.x & 63, c0 = from(), c1 = to();
         const uint64_t below = (1ull << lane) - 1;
-        const int c0 = from(wave), c1 = min(c0 + part(), row.n);
+        const auto in = [&](float x) { return x >= floor && x > -INFINITY; };
         int count = 0;
 #pragma unroll 1
         for (int c = c0; c < c1; c += 256) {                        // all lanes of a wave go round together
             float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             if (c + lane * 4 < c1) row.four(c + lane * 4, x);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) count += __popcll(__builtin_amdgcn_ballot_w64(kept(x[i], c + lane * 4 + i)));
+            for (int i = 0; i < 4; ++i) count += __popcll(__builtin_amdgcn_ballot_w64(in(x[i])));
         }
-        if (lane == 0) s.redi[wave] = count;
+        if (lane == 0) s.redi[wave()] = count;
         __syncthreads();
         int at = 0, many = 0;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            at += w < wave ? s.redi[w] : 0;
+            at += w < wave() ? s.redi[w] : 0;
             many += s.redi[w];
         }
-        __syncthreads();
-        if (many > L::KEPT) return false;
+        if (many <= L::KEPT) {
 #pragma unroll 1
-        for (int c = c0; c < c1; c += 256) {
-            float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            if (c + lane * 4 < c1) row.four(c + lane * 4, x);
-            int place = at;
-            bool in[4];
+            for (int c = c0; c < c1 && count; c += 256) {
+                float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if (c + lane * 4 < c1) row.four(c + lane * 4, x);
+                int place = at;
+                bool take[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                in[i] = kept(x[i], c + lane * 4 + i);
-                const uint64_t m = __builtin_amdgcn_ballot_w64(in[i]);
-                place += __popcll(m & below);
-                at += __popcll(m);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (in[i]) {
-                    s.kept_x[place] = Score<DT>::narrow(x[i]);
-                    s.kept_i[place++] = c + lane * 4 + i;
+                for (int i = 0; i < 4; ++i) {
+                    take[i] = in(x[i]);
+                    const uint64_t m = __builtin_amdgcn_ballot_w64(take[i]);
+                    place += __popcll(m & below);
+                    at += __popcll(m);
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (take[i]) {
+                        s.kept_x[place] = Score<DT>::narrow(x[i]);
+                        s.kept_i[place++] = c + lane * 4 + i;
+                    }
+            }
+            if (threadIdx.x < (unsigned)(-many & 3)) s.kept_x[many + threadIdx.x] = Score<DT>::narrow(-INFINITY);      // to whole quads
         }
-        if (threadIdx.x < (unsigned)(-many & 3)) s.kept_x[many + threadIdx.x] = Score<DT>::narrow(-INFINITY);      // to whole quads
         __syncthreads();
-        row.p = s.kept_x;
-        row.n = many;
-        cut_x = -INFINITY;
-        cut_i = -1;
-        return true;
+        return many;
     }
 };
+
+// The lower end (a score's key, its low 16 bits cleared) of what at least `need` of the wave's lanes have: bit by bit from the top.
+__device__ __forceinline__ uint32_t lanes_above(uint32_t key, int need)
+{
+    uint32_t t = 0;
+#pragma unroll
+    for (int b = 31; b >= 16; --b) {
+        const uint32_t with = t | 1u << b;
+        if (__popcll(__builtin_amdgcn_ballot_w64(key >= with)) >= need) t = with;
+    }
+    return t;
+}
 
 template <int DT, bool STAGED, int W>
 __global__ __launch_bounds__(64 * W, 6) void sample_kernel(const SampleArgs a)
 {
     typedef Score<DT> S;
+    typedef Lds<DT, W> L;
     constexpr int NT = 64 * W;
     extern __shared__ __attribute__((aligned(16))) char staged[];
-    __shared__ Lds<DT, W> s;
+    __shared__ L s;
     const int64_t n = blockIdx.x;
-    const int V = a.V, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int V = a.V, tid = threadIdx.x, wave = tid >> 6;
     const auto answer = [&](int64_t i, float lp) {
         a.idx[n] = i;
         if (a.logp) a.logp[n] = lp;
@@ -507,47 +592,58 @@ __global__ __launch_bounds__(64 * W, 6) void sample_kernel(const SampleArgs a)
     }
     const typename S::Raw *z = reinterpret_cast<const typename S::Raw *>(a.z) + n * a.ld;
     typename S::Raw *lds = reinterpret_cast<typename S::Raw *>(staged);
-    Draw<DT, STAGED, W> d(s);
-    d.row = {z, V, false};
-    d.cut_x = -INFINITY;
-    d.cut_i = -1;                                                   // nothing with a score of -inf
-    float mx = -INFINITY;
-    if (STAGED) {
-        const View<DT, false> from{z, V, false};
-#pragma unroll 4
-        for (int c = tid * 4; c < V; c += NT * 4) {
-            float x[4];
-            from.four(c, x);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                mx = fmaxf(mx, x[i]);
-                lds[c + i] = S::narrow(x[i]);
-            }
-        }
-        d.row.p = lds;
-    } else {
-        d.each([&](float v, int) { mx = fmaxf(mx, v); });
-    }
     const double T = a.temperature ? (double)a.temperature[n] : a.t0, P = a.top_p ? (double)a.top_p[n] : a.p0;
     const double mp = a.min_p ? (double)a.min_p[n] : a.m0;
-    const int k = a.top_k ? a.top_k[n] : a.k0;
+    int k = a.top_k ? a.top_k[n] : a.k0;
+    k = k < V ? k : 0;                                              // 0 and below: all
     const float u = a.u[n];
-    float own = mx;
-    mx = block_max_f32<W>(mx, s.redf);
+    View<DT, STAGED> row = {STAGED ? lds : z, V, false};
+    float own = -INFINITY;                                          // the thread's maximum
+    const View<DT, false> from{z, V, false};
+#pragma unroll 4
+    for (int c = tid * 4; c < V; c += NT * 4) {
+        float x[4];
+        from.four(c, x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            own = fmaxf(own, x[i]);
+            if (STAGED) lds[c + i] = S::narrow(x[i]);
+        }
+    }
+    // The row's maximum, and a score that at least k codes reach: k / W of each wave's own maxima do.
+    const int each = (k + W - 1) / W;
+    const bool bounded = STAGED && k > 0 && each <= 64;
+    const float wmax = wave_max(own);
+    const uint32_t key = bounded ? lanes_above(key_of(own), each) : 0;
+    if ((tid & 63) == 0) {
+        s.redf[wave] = wmax;
+        s.redi[wave] = (int)key;
+    }
+    __syncthreads();
+    float mx = s.redf[0];
+    uint32_t low = (uint32_t)s.redi[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+        mx = fmaxf(mx, s.redf[w]);
+        low = min(low, (uint32_t)s.redi[w]);
+    }
+    __syncthreads();
     if (mx == -INFINITY) {
         if (tid == 0) answer(-1, 0.f);
         return;
     }
+    float floor = low >= key_of(-INFINITY) ? score_of(low) : -INFINITY;
     if (mx == INFINITY) {
         mx = 0.f;
-        own = own == INFINITY ? 0.f : -INFINITY;
+        floor = -INFINITY;
         if (STAGED) {
             for (int c = tid; c < (V + 3) / 4 * 4; c += NT) lds[c] = S::narrow(S::widen(lds[c]) == INFINITY ? 0.f : -INFINITY);
+            __syncthreads();
         } else {
-            d.row.inf = true;
+            row.inf = true;
         }
     }
-    __syncthreads();
+    Draw<DT, STAGED, W, L> d(s, row);
     if (!(T > 0.0)) {                                               // the lowest index that has the maximum
         int first = INT32_MAX;
         d.each([&](float v, int c) { first = v == mx && c < first ? c : first; });
@@ -556,66 +652,30 @@ __global__ __launch_bounds__(64 * W, 6) void sample_kernel(const SampleArgs a)
         return;
     }
     const Row r{(double)mx, fmin(1.0 / T, 1e300), ldexp(1.0, a.shift), mp > 1.0 ? 1.0 : mp};
-    const auto units = [&](float v) { return r.template units<false>(v); };
-    bool listed = false;
-    if (k > 0 && k < V) {
-        d.find_cut(mx, (uint64_t)k, d.limit_of(mx, own, k), [](float) { return (uint64_t)1; });
-        if (k <= Lds<DT, W>::KEPT) listed = d.compact();
-    }
-    if (P < 1.0) {
-        const double Z = (double)block_sum_u64<W>(d.sum(units), s.red), g = ceil(P * Z);
-        // codes further than D from the maximum have at most n exp(-D / T) = (1 - P) Z together
-        const float D = (float)(T * 1.0001 * log((double)d.row.n * r.scale / ((1.0 - P) * Z)));
-        d.find_cut(mx, g > 1.0 ? (uint64_t)g : 1, D > 0.f ? Bins<Lds<DT, W>::BINS>::of(D) : 0, units);      // kept while less than that lies before them
-        if (!listed) listed = d.compact();
-    }
-    // the draw: the waves' sums, then the wave that it falls to goes over its part again
-    // (NaN min_p: nothing is under it)
-    const auto drawn = [&](float v) { return r.min_p > 0.0 ? r.template units<true>(v) : r.template units<false>(v); };
-    uint64_t part = d.sum(drawn);
-    part = wave_sum_u64(part);
-    if (lane == 0) s.red[wave] = part;
-    __syncthreads();
+    // Where a bound says that the first cut lies among few codes, those become a list and one wave does the rest on it, without barriers; the
+    // others make room for the next row.
     uint64_t Z = 0;
-#pragma unroll
-    for (int w = 0; w < W; ++w) Z += s.red[w];
-    const double t = floor((double)(u > 0.f ? u : 0.f) * (double)Z);
-    uint64_t target = t < (double)Z ? (uint64_t)t : Z - 1;
-    if (target >= Z) target = Z - 1;
-    uint64_t before = 0;
-    int mine = 0;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-        const uint64_t here = s.red[w];
-        if (before + here <= target) {
-            before += here;
-            mine = w + 1;
-        } else {
-            break;
+    bool narrow = bounded;
+    if (STAGED && k <= 0 && P < 1.0) {
+        Z = d.total(d.sum([&](float v) { return r.units(v); }));
+        // The codes further than D from the maximum have at most V (exp(-D / T) 2^shift + 1) units.  That much may be missing of (1 - P) Z, less what
+        // rounding P Z and Z to f64 takes.
+        const double spare = (1.0 - P) * (double)Z * 0.999 - (double)V - 4096.0;
+        if (spare > 0.0) {
+            const double D = T * log((double)V * r.scale / spare);
+            narrow = D < 1e30;
+            floor = (float)((double)mx - fmax(D, 0.0) - fabs((double)mx) * 1e-6 - 1e-30);
         }
     }
-    if (wave != mine) return;
-    const int c0 = d.from(wave), c1 = min(c0 + d.part(), d.row.n);
-#pragma unroll 1
-    for (int c = c0; c < c1; c += 256) {                            // the wave's lanes go round together
-        float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        const int at = c + lane * 4;
-        if (at < c1) d.row.four(at, x);
-        uint64_t q[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) q[i] = d.kept(x[i], at + i) ? drawn(x[i]) : 0;
-        const uint64_t sum = (q[0] + q[1]) + (q[2] + q[3]), upto = wave_scan<unsigned long long>(sum) + before;
-        if (upto > target && upto - sum <= target) {
-            uint64_t b = upto - sum;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (b <= target && b + q[i] > target) answer(listed ? s.kept_i[at + i] : at + i, a.logp ? r.logp(x[i], Z) : 0.f);
-                b += q[i];
-            }
+    if (STAGED && narrow) {
+        const int many = d.compact(floor);
+        if (many <= L::KEPT) {
+            if (wave) return;
+            Draw<DT, true, 1, L>(s, View<DT, true>{s.kept_x, many, false}).finish(r, mx, k, P, u, Z, [&](int c, float x, uint64_t mass) { answer(s.kept_i[c], a.logp ? r.logp(x, mass) : 0.f); });
+            return;
         }
-        before = __shfl((unsigned long long)upto, 63, 64);
-        if (before > target) return;
     }
+    d.finish(r, mx, k, P, u, Z, [&](int c, float x, uint64_t mass) { answer(c, a.logp ? r.logp(x, mass) : 0.f); });
 }
 
 }  // namespace mq
