@@ -20,6 +20,8 @@
 // one over that bin's lower bits narrows it, and the few codes left are put into a list and counted against each other.  Where that list
 // overflows (hundreds of equal scores across the cut) radix selection over the bits of the score finds the cut instead.
 // A wave covers a contiguous part of the row, so that sums up to a code need one number per wave.
+#include <algorithm>
+
 #include "common.h"
 
 namespace mq {
@@ -36,27 +38,41 @@ struct SampleArgs {
     const uint8_t *padded;
     int64_t *idx;
     float *logp;
+    int64_t rows;
+    __device__ __forceinline__ double T(int64_t n) const { return temperature ? (double)temperature[n] : t0; }
+    __device__ __forceinline__ double P(int64_t n) const { return top_p ? (double)top_p[n] : p0; }
+    __device__ __forceinline__ double min(int64_t n) const { return min_p ? (double)min_p[n] : m0; }
+    __device__ __forceinline__ int k(int64_t n) const
+    {
+        const int v = top_k ? top_k[n] : k0;
+        return v < V ? v : 0;                                        // 0 and below: all
+    }
 };
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint16_t u16x4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4a __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x4a __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ float clean(float x) { return x == x ? x + 0.0f : -INFINITY; }      // NaN is never drawn; -0 and +0 are one score
+__device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY); }      // NaN is never drawn
 template <int DT> struct Score;                                      // 0 f32, 1 bf16, 2 f16, as they lie in memory
 template <> struct Score<0> {
     typedef float Raw;
     typedef f32x4u Raw4;
+    typedef f32x4a Quad;                                             // in LDS
     static __device__ __forceinline__ float widen(Raw v) { return v; }
     static __device__ __forceinline__ Raw narrow(float v) { return v; }
 };
 template <> struct Score<1> {
     typedef uint16_t Raw;
     typedef u16x4u Raw4;
+    typedef u16x4a Quad;
     static __device__ __forceinline__ float widen(Raw v) { return __uint_as_float((uint32_t)v << 16); }
     static __device__ __forceinline__ Raw narrow(float v) { return (Raw)(__float_as_uint(v) >> 16); }      // of a value that is one
 };
 template <> struct Score<2> {
     typedef uint16_t Raw;
     typedef u16x4u Raw4;
+    typedef u16x4a Quad;
     static __device__ __forceinline__ float widen(Raw v) { return (float)__builtin_bit_cast(_Float16, v); }
     static __device__ __forceinline__ Raw narrow(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
 };
@@ -76,16 +92,18 @@ struct View {
     }
     __device__ __forceinline__ void four(int c, float (&x)[4]) const      // c is a multiple of 4 below n
     {
-        if (STAGED || c + 4 <= n) {
+        if (STAGED) {
+            const typename S::Quad q = *reinterpret_cast<const typename S::Quad *>(p + c);
+            const typename S::Raw v[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = S::widen(v[i]);
+        } else if (c + 4 <= n) {
             const typename S::Raw4 q = *reinterpret_cast<const typename S::Raw4 *>(p + c);
             const typename S::Raw v[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                x[i] = S::widen(v[i]);
-                if (!STAGED) {
-                    x[i] = clean(x[i]);
-                    if (inf) x[i] = x[i] == INFINITY ? 0.f : -INFINITY;
-                }
+                x[i] = clean(S::widen(v[i]));
+                if (inf) x[i] = x[i] == INFINITY ? 0.f : -INFINITY;
             }
         } else {
 #pragma unroll
@@ -94,42 +112,42 @@ struct View {
     }
 };
 
-// exp(d), -746 <= d <= 0, in f64: d = n ln 2 + r, |r| <= 0.35, Taylor's series of exp(r) to r^11 (the rest is under 1e-14).
-constexpr double LN2_HI = 2977044472.0 / 4294967296.0, LN2_LO = -4.2009150726810846e-11;    // ln 2 2^32 to the nearest whole number, and the rest
-__device__ __forceinline__ double exp_neg(double d)
+// 2^r, |r| <= 1/2, in f64: 1 + r q(r), q by interpolation at Chebyshev's points; relative error under 4e-14, 1 at 0.  (Taylor's series needs two
+// more terms, and the masses are what limits the filters of a whole row: about 25 operations in f64 a code, at the rate of f32.)
+__device__ __forceinline__ double exp2_half(double r)
 {
-    const double n = rint(d * 1.4426950408889634074);
-    double r = fma(n, -LN2_HI, d);                                  // exact: LN2_HI has 32 bits, n 11
-    r = fma(n, -LN2_LO, r);
-    double p = 1.0 / 39916800.0;
-    p = fma(p, r, 1.0 / 3628800.0);
-    p = fma(p, r, 1.0 / 362880.0);
-    p = fma(p, r, 1.0 / 40320.0);
-    p = fma(p, r, 1.0 / 5040.0);
-    p = fma(p, r, 1.0 / 720.0);
-    p = fma(p, r, 1.0 / 120.0);
-    p = fma(p, r, 1.0 / 24.0);
-    p = fma(p, r, 1.0 / 6.0);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
-    return ldexp(p, (int)n);
+    double q = 1.0203121063391729e-07;
+    q = fma(q, r, 1.3255224878668817e-06);
+    q = fma(q, r, 1.525268684626772e-05);
+    q = fma(q, r, 1.5403455852453838e-04);
+    q = fma(q, r, 1.3333558179043112e-03);
+    q = fma(q, r, 9.618129159402558e-03);
+    q = fma(q, r, 5.5504108664760424e-02);
+    q = fma(q, r, 2.402265069581299e-01);
+    q = fma(q, r, 6.931471805599453e-01);
+    return fma(q, r, 1.0);
 }
 // What of a row's settings the weights need; max is finite (rows with +inf are remapped to scores 0 and -inf before)
 struct Row {
     double max, per_t;                   // 1 / T; 0 for T = inf
-    double scale;                        // 2^shift
-    double min_p;                        // <= 1
-    // Units of a code with a score above -inf: w 2^shift to the nearest whole number, at least 1 - the bits of w 2^shift + 2^52 (shift <= 51,
-    // w <= 1); 0 where w would underflow and where it is under `least`.
-    __device__ __forceinline__ uint64_t units(float x, double least = 0.0) const
+    double per2;                         // log2(e) / T
+    int shift;                           // weights are w 2^shift
+    double least;                        // min_p 2^shift, min_p <= 1
+    __device__ __forceinline__ Row(float max_, double T, double min_p, int shift_)
+        : max((double)max_), per_t(fmin(1.0 / T, 1e300)), per2(per_t * 1.4426950408889634074), shift(shift_), least(ldexp(min_p > 1.0 ? 1.0 : min_p, shift_))
     {
-        const double d = ((double)x - max) * per_t, w = exp_neg(fmax(d, -746.0));
-        const uint64_t q = (uint64_t)__double_as_longlong(fma(w, scale, 4503599627370496.0)) & 0xfffffffffffffull;
-        return d < -745.0 || w < least ? 0 : q > 1 ? q : 1;
+    }
+    // Units of a code with a score above -inf: w 2^shift to the nearest whole number, at least 1 - the bits of w 2^shift + 2^52 (shift <= 51,
+    // w <= 1); 0 where w would underflow in f64 and where w 2^shift is under `limit`.
+    __device__ __forceinline__ uint64_t units(float x, double limit = 0.0) const
+    {
+        const double d = ((double)x - max) * per2, c = fmax(d, -1100.0), n = rint(c);
+        const double w = ldexp(exp2_half(c - n), (int)n + shift);
+        const uint64_t q = (uint64_t)__double_as_longlong(fmax(w, 1.0) + 4503599627370496.0) & 0xfffffffffffffull;
+        return d < -1074.8 || w < limit ? 0 : q;
     }
     // log of a weight's share of Z units
-    __device__ __forceinline__ float logp(float x, uint64_t Z) const { return (float)(((double)x - max) * per_t - log((double)Z / scale)); }
+    __device__ __forceinline__ float logp(float x, uint64_t Z) const { return (float)(((double)x - max) * per_t - log(ldexp((double)Z, -shift))); }
 };
 
 // Inclusive scans over the 64 lanes by DPP (row shifts, then the rows' last lanes broadcast): a tenth of the latency of the LDS crossbar's.
@@ -210,7 +228,7 @@ __device__ __forceinline__ void find_bin(const U *hist, uint64_t goal, Found *ou
 // order-preserving key of a score
 __device__ __forceinline__ uint32_t key_of(float x)
 {
-    const uint32_t b = __float_as_uint(x);
+    const uint32_t b = __float_as_uint(x + 0.0f);                   // -0 and +0 are one score
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 __device__ __forceinline__ float score_of(uint32_t key) { return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key); }
@@ -220,14 +238,12 @@ __device__ __forceinline__ float score_of(uint32_t key) { return __uint_as_float
 // An inner bin holds distances that differ in their lower SH bits only; its own bins are the highest of those.
 template <int BINS>
 struct Bins {
-    static constexpr int LOG = BINS == 512 ? 9 : 8, SH = 28 - LOG;
+    static constexpr int LOG = BINS == 512 ? 9 : BINS == 256 ? 8 : 7, SH = 28 - LOG;
     static __device__ __forceinline__ int of(float d)
     {
         const int b = (int)(__float_as_uint(d) >> SH) - ((127 - 12) << (23 - SH));
         return min(max(b, 0), BINS - 1);
     }
-    // the largest distance in bin b (of an inner one)
-    static __device__ __forceinline__ float end(int b) { return __uint_as_float((uint32_t)(b + 1 + ((127 - 12) << (23 - SH))) << SH) * 0.99999994f; }
     static __device__ __forceinline__ int inner(float d) { return (int)(__float_as_uint(d) >> (SH - LOG)) & (BINS - 1); }
 };
 
@@ -239,17 +255,36 @@ struct Entry {
     int i;
     unsigned long long w;
 };
-template <int DT, int W>
-struct Lds {
-    static constexpr int BINS = W <= 2 ? 256 : 512, LIST = BINS / 2, KEPT = W <= 2 ? 256 : W <= 4 ? 512 : 1024;
+// What a cut is found with
+template <int NBINS>
+struct Search {
+    static constexpr int BINS = NBINS, LIST = NBINS / 2;
     unsigned long long hist[BINS];
     Entry list[LIST];                                               // codes of the bin that a cut falls into
-    alignas(16) typename Score<DT>::Raw kept_x[KEPT];               // the kept codes in index order, once they are few
-    int kept_i[KEPT];
-    unsigned long long red[W];
-    float redf[W], cut_x;
-    int redi[W], cut_i, length;
+    float cut_x;
+    int cut_i, length;
     Found found;
+};
+// The codes kept of a row, in index order, once they are few, and the row's settings
+template <int DT, int KEPT>
+struct Few {
+    alignas(16) typename Score<DT>::Raw x[KEPT];
+    uint16_t i[KEPT];                                               // a row in LDS has at most 16384
+    double T, P, min_p;
+    int k, padded;
+    float u;
+    float max;
+    int state;                                                      // the number of codes kept, or
+    enum { DONE = -1, WHOLE = -2 };                                 // answered; to be worked on by the whole block
+};
+// A block's LDS next to the row
+template <int W, int NBINS>
+struct Shared {
+    static constexpr int BINS = NBINS;
+    Search<BINS> search;
+    unsigned long long red[W];
+    float redf[W];
+    int redi[W], counts[W];
 };
 
 // W waves of a block work together on a row; with W = 1 one wave works on by itself, the others have left.
@@ -263,23 +298,30 @@ __device__ __forceinline__ void together()
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
 }
-// L: the block's LDS (of its own number of waves)
-template <int DT, bool STAGED, int W, typename L>
+template <int DT, bool STAGED, int W, int BINS>
 struct Draw {
     static constexpr int NT = 64 * W, FEW = 40;
-    typedef Bins<L::BINS> B;
-    L &s;
+    typedef Bins<BINS> B;
+    Search<BINS> &s;
+    unsigned long long *red;                                        // W each
+    int *redi;
     View<DT, STAGED> row;
     float cut_x;                                                    // kept: at or before (cut_x, cut_i) in the order
     int cut_i;
 
-    __device__ __forceinline__ Draw(L &s_, const View<DT, STAGED> &v) : s(s_), row(v), cut_x(-INFINITY), cut_i(-1) {}      // nothing with a score of -inf
+    __device__ __forceinline__ Draw(Search<BINS> &s_, unsigned long long *red_, int *redi_, const View<DT, STAGED> &v) : s(s_), red(red_), redi(redi_), row(v), cut_x(-INFINITY), cut_i(-1) {}      // nothing with a score of -inf
     // The wave's part of the row: codes [from, to), a multiple of 256 from the last one's
     __device__ __forceinline__ int wave() const { return W > 1 ? (int)(threadIdx.x >> 6) : 0; }
     __device__ __forceinline__ int part() const { return (row.n + 256 * W - 1) / (256 * W) * 256; }
     __device__ __forceinline__ int from() const { return wave() * part(); }
     __device__ __forceinline__ int to() const { return min(from() + part(), row.n); }
     __device__ __forceinline__ bool kept(float x, int c) const { return x > cut_x || (x == cut_x && c <= cut_i); }
+    // all codes with scores from x up may be kept
+    __device__ __forceinline__ void from_score(float x)
+    {
+        cut_x = x;
+        cut_i = x > -INFINITY ? INT32_MAX : -1;
+    }
     // f(x, c) for the kept codes, one at a time: a small loop, there are several of them and the instruction cache is shared
     template <typename F>
     __device__ __forceinline__ void each(F f) const
@@ -317,34 +359,35 @@ struct Draw {
     template <typename Q>
     __device__ __forceinline__ void find_cut_by_bits(uint64_t goal, Q q)
     {
-        uint32_t prefix = 0;
-        uint64_t above = 0;
+        uint64_t prefix = 0, above = 0;
 #pragma unroll 1
-        for (int sh = 24; sh >= 0; sh -= 8) {
+        for (int sh = 32; sh > 0;) {
+            const int bits = min(B::LOG, sh);
+            sh -= bits;
             together<W>();
-            for (int b = (threadIdx.x & (NT - 1)); b < 256; b += NT) s.hist[b] = 0;
+            for (int b = (W > 1 ? (int)threadIdx.x : (int)threadIdx.x & 63); b < BINS; b += NT) s.hist[b] = 0;
             together<W>();
             each([&](float v, int) {
                 const uint32_t key = key_of(v);
-                if (sh == 24 || key >> (sh + 8) == prefix) atomicAdd(&s.hist[(key >> sh) & 255u], (unsigned long long)q(v));
+                if ((uint64_t)key >> (sh + bits) == prefix) atomicAdd(&s.hist[(key >> sh) & ((1u << bits) - 1u)], (unsigned long long)q(v));
             });
             together<W>();
-            find_bin<256, true, W>(s.hist, goal - above, &s.found);
-            prefix = prefix << 8 | (uint32_t)s.found.bin;
+            find_bin<BINS, true, W>(s.hist, goal - above, &s.found);
+            prefix = prefix << bits | (uint64_t)s.found.bin;
             above += s.found.before;
         }
         // codes with the border's score are kept while above + j w < goal: the last of them by its index
-        const float border = score_of(prefix);
+        const float border = score_of((uint32_t)prefix);
         const uint64_t w = q(border);
         const int need = (int)((goal - above + w - 1) / w);
         const int lane = threadIdx.x & 63, c0 = from(), c1 = to();
         uint32_t mine = 0;
         each([&](float v, int) { mine += v == border; });
         const int count = (int)wave_total(mine);
-        if (lane == 0) s.redi[wave()] = count;
+        if (lane == 0) redi[wave()] = count;
         together<W>();
         int before = 0;
-        for (int v = 0; v < wave(); ++v) before += s.redi[v];
+        for (int v = 0; v < wave(); ++v) before += redi[v];
         if (before < need && before + count >= need) {
 #pragma unroll 1
             for (int c = c0; c < c1; c += 256) {                    // the wave's lanes go round together
@@ -371,14 +414,14 @@ struct Draw {
     template <typename Q>
     __device__ __forceinline__ bool find_cut(float mx, uint64_t goal, Q q)
     {
-        const int tid = threadIdx.x & (NT - 1);
+        const int tid = (W > 1 ? (int)threadIdx.x : (int)threadIdx.x & 63);
         int bin = 0, sub = -1;
         uint64_t above = 0;
 #pragma unroll 1
         for (int level = 0; level < 2; ++level) {
             together<W>();
 #pragma unroll 1
-            for (int b = tid; b < L::BINS; b += NT) s.hist[b] = 0;
+            for (int b = tid; b < BINS; b += NT) s.hist[b] = 0;
             if (tid == 0) s.length = 0;
             together<W>();
             each([&](float v, int) {
@@ -387,7 +430,7 @@ struct Draw {
                 if (level == 0 || b == bin) atomicAdd(&s.hist[level == 0 ? b : B::inner(d)], (unsigned long long)q(v));
             });
             together<W>();
-            find_bin<L::BINS, false, W>(s.hist, goal - above, &s.found);
+            find_bin<BINS, false, W>(s.hist, goal - above, &s.found);
             if (level == 0) {
                 if (s.found.total < goal) return false;
                 bin = s.found.bin;
@@ -399,13 +442,13 @@ struct Draw {
                 const float d = mx - v;
                 if (B::of(d) != bin || (sub >= 0 && B::inner(d) != sub)) return;
                 const int e = atomicAdd(&s.length, 1);
-                if (e < L::LIST) s.list[e] = Entry{v, c, (unsigned long long)q(v)};
+                if (e < s.LIST) s.list[e] = Entry{v, c, (unsigned long long)q(v)};
             });
             together<W>();
-            if (s.length <= FEW || bin == 0 || bin == L::BINS - 1) break;
+            if (s.length <= FEW || bin == 0 || bin == BINS - 1) break;
         }
         const int many = s.length;
-        if (many > L::LIST) {
+        if (many > s.LIST) {
             find_cut_by_bits(goal, q);
             return true;
         }
@@ -446,13 +489,13 @@ struct Draw {
             find_cut(mx, goal, [&](float v) { return stage == 0 ? (uint64_t)1 : r.units(v); });
         }
         // the waves' sums, then the wave that the draw falls to goes over its part again (NaN min_p: nothing is under it)
-        const uint64_t part_ = wave_total(sum([&](float v) { return r.units(v, r.min_p); }));
+        const uint64_t part_ = wave_total(sum([&](float v) { return r.units(v, r.least); }));
         together<W>();
-        if (lane == 0) s.red[wave()] = part_;
+        if (lane == 0) red[wave()] = part_;
         together<W>();
         uint64_t mass = 0;
 #pragma unroll
-        for (int w = 0; w < W; ++w) mass += s.red[w];
+        for (int w = 0; w < W; ++w) mass += red[w];
         const double t = floor((double)(u > 0.f ? u : 0.f) * (double)mass);
         uint64_t target = t < (double)mass ? (uint64_t)t : mass - 1;
         if (target >= mass) target = mass - 1;
@@ -460,7 +503,7 @@ struct Draw {
         int mine = 0;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            const uint64_t here = s.red[w];
+            const uint64_t here = red[w];
             if (before + here <= target) {
                 before += here;
                 mine = w + 1;
@@ -477,7 +520,7 @@ struct Draw {
             if (at < c1) row.four(at, x);
             uint64_t q[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q[i] = kept(x[i], at + i) ? r.units(x[i], r.min_p) : 0;
+            for (int i = 0; i < 4; ++i) q[i] = kept(x[i], at + i) ? r.units(x[i], r.least) : 0;
             const uint64_t four = (q[0] + q[1]) + (q[2] + q[3]), upto = wave_scan(four) + before;
             if (upto > target && upto - four <= target) {
                 uint64_t b = upto - four;
@@ -497,11 +540,11 @@ struct Draw {
         v = wave_total(v);
         if (W == 1) return v;
         __syncthreads();
-        if ((threadIdx.x & 63) == 0) s.red[threadIdx.x >> 6] = v;
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
         uint64_t t = 0;
 #pragma unroll
-        for (int w = 0; w < W; ++w) t += s.red[w];
+        for (int w = 0; w < W; ++w) t += red[w];
         return t;
     }
     // codes are kept while less than this lies before them
@@ -511,11 +554,11 @@ struct Draw {
         return g > 1.0 ? (uint64_t)g : 1;
     }
     // Puts the codes with x >= floor into the list of kept codes, in index order, where they are at most KEPT.  How many they are.
-    __device__ __forceinline__ int compact(float floor)
+    template <int KEPT>
+    __device__ __forceinline__ int compact(float floor, Few<DT, KEPT> &few)
     {
         const int lane = threadIdx.x & 63, c0 = from(), c1 = to();
-        const uint64_t below = (1ull << lane) - 1;
-        const auto in = [&](float x) { return x >= floor && x > -INFINITY; };
+        const auto in = [&](float v) { return v >= floor && v > -INFINITY; };
         int count = 0;
 #pragma unroll 1
         for (int c = c0; c < c1; c += 256) {                        // all lanes of a wave go round together
@@ -524,38 +567,35 @@ struct Draw {
 #pragma unroll
             for (int i = 0; i < 4; ++i) count += __popcll(__builtin_amdgcn_ballot_w64(in(x[i])));
         }
-        if (lane == 0) s.redi[wave()] = count;
-        __syncthreads();
+        if (lane == 0) redi[wave()] = count;
+        together<W>();
         int at = 0, many = 0;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            at += w < wave() ? s.redi[w] : 0;
-            many += s.redi[w];
+            at += w < wave() ? redi[w] : 0;
+            many += redi[w];
         }
-        if (many <= L::KEPT) {
+        if (many <= KEPT) {
 #pragma unroll 1
             for (int c = c0; c < c1 && count; c += 256) {
                 float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 if (c + lane * 4 < c1) row.four(c + lane * 4, x);
                 int place = at;
-                bool take[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    take[i] = in(x[i]);
-                    const uint64_t m = __builtin_amdgcn_ballot_w64(take[i]);
-                    place += __popcll(m & below);
+                    const uint64_t m = __builtin_amdgcn_ballot_w64(in(x[i]));
+                    place += (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
                     at += __popcll(m);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (take[i]) {
-                        s.kept_x[place] = Score<DT>::narrow(x[i]);
-                        s.kept_i[place++] = c + lane * 4 + i;
+                    if (in(x[i])) {
+                        few.x[place] = Score<DT>::narrow(x[i]);
+                        few.i[place++] = (uint16_t)(c + lane * 4 + i);
                     }
             }
-            if (threadIdx.x < (unsigned)(-many & 3)) s.kept_x[many + threadIdx.x] = Score<DT>::narrow(-INFINITY);      // to whole quads
+            if (threadIdx.x < (unsigned)(-many & 3)) few.x[many + threadIdx.x] = Score<DT>::narrow(-INFINITY);      // to whole quads
         }
-        __syncthreads();
         return many;
     }
 };
@@ -572,16 +612,56 @@ __device__ __forceinline__ uint32_t lanes_above(uint32_t key, int need)
     return t;
 }
 
+// The block's maximum, and a score that at least k codes reach where HELD and k <= 64 W: k / W of each wave's own maxima do.  own: the thread's.
+template <int W>
+__device__ __forceinline__ float maximum(float own, int k, bool bounded, float *redf, int *redi, float *floor)
+{
+    const int wave = W > 1 ? threadIdx.x >> 6 : 0;
+    const float wmax = wave_max(own);
+    uint32_t low = bounded ? lanes_above(key_of(own), (k + W - 1) / W) : 0;
+    float mx = wmax;
+    if (W > 1) {
+        if ((threadIdx.x & 63) == 0) {
+            redf[wave] = wmax;
+            redi[wave] = (int)low;
+        }
+        __syncthreads();
+        mx = redf[0];
+        low = (uint32_t)redi[0];
+#pragma unroll
+        for (int w = 1; w < W; ++w) {
+            mx = fmaxf(mx, redf[w]);
+            low = min(low, (uint32_t)redi[w]);
+        }
+    }
+    *floor = low >= key_of(-INFINITY) ? score_of(low) : -INFINITY;
+    return mx;
+}
+// The lowest index with the maximum
 template <int DT, bool STAGED, int W>
-__global__ __launch_bounds__(64 * W, 6) void sample_kernel(const SampleArgs a)
+__device__ __forceinline__ int first_of(float mx, float own, const View<DT, STAGED> &row, int c0, int c1, float *redf)
+{
+    int first = 1 << 24;                                            // indices are below
+    if (own == mx) {
+#pragma unroll 1
+        for (int c = c0; c < c1 && first == 1 << 24; c += 256) {
+            float y[4];
+            row.four(c, y);
+#pragma unroll
+            for (int i = 3; i >= 0; --i) first = y[i] == mx ? c + i : first;
+        }
+    }
+    together<W>();
+    return (int)-block_max_f32<W>(-(float)first, redf);
+}
+
+// One row by a block of W waves.  HELD: it is read once, into LDS (at `lds`), each wave's part by itself; else each time from memory.  few: NULL,
+// or where a list of codes may go.
+template <int DT, bool HELD, int W, typename H, int KEPT>
+__device__ __forceinline__ void draw_row(const SampleArgs &a, int64_t n, typename Score<DT>::Raw *lds, H &s, Few<DT, KEPT> *few)
 {
     typedef Score<DT> S;
-    typedef Lds<DT, W> L;
-    constexpr int NT = 64 * W;
-    extern __shared__ __attribute__((aligned(16))) char staged[];
-    __shared__ L s;
-    const int64_t n = blockIdx.x;
-    const int V = a.V, tid = threadIdx.x, wave = tid >> 6;
+    const int V = a.V, tid = threadIdx.x, lane = tid & 63;
     const auto answer = [&](int64_t i, float lp) {
         a.idx[n] = i;
         if (a.logp) a.logp[n] = lp;
@@ -590,92 +670,176 @@ __global__ __launch_bounds__(64 * W, 6) void sample_kernel(const SampleArgs a)
         if (tid == 0) answer(-1, 0.f);
         return;
     }
+    const double T = a.T(n), P = a.P(n);
+    const int k = a.k(n);
     const typename S::Raw *z = reinterpret_cast<const typename S::Raw *>(a.z) + n * a.ld;
-    typename S::Raw *lds = reinterpret_cast<typename S::Raw *>(staged);
-    const double T = a.temperature ? (double)a.temperature[n] : a.t0, P = a.top_p ? (double)a.top_p[n] : a.p0;
-    const double mp = a.min_p ? (double)a.min_p[n] : a.m0;
-    int k = a.top_k ? a.top_k[n] : a.k0;
-    k = k < V ? k : 0;                                              // 0 and below: all
-    const float u = a.u[n];
-    View<DT, STAGED> row = {STAGED ? lds : z, V, false};
-    float own = -INFINITY;                                          // the thread's maximum
+    Draw<DT, HELD, W, H::BINS> d(s.search, s.red, s.counts, View<DT, HELD>{HELD ? lds : z, V, false});
     const View<DT, false> from{z, V, false};
+    const int c0 = d.from() + lane * 4, c1 = d.to();
+    float own = -INFINITY;
 #pragma unroll 4
-    for (int c = tid * 4; c < V; c += NT * 4) {
+    for (int c = c0; c < c1; c += 256) {
         float x[4];
         from.four(c, x);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            own = fmaxf(own, x[i]);
-            if (STAGED) lds[c + i] = S::narrow(x[i]);
-        }
+        for (int i = 0; i < 4; ++i) own = fmaxf(own, x[i]);
+        if (HELD) *reinterpret_cast<typename S::Quad *>(lds + c) = typename S::Quad{S::narrow(x[0]), S::narrow(x[1]), S::narrow(x[2]), S::narrow(x[3])};
     }
-    // The row's maximum, and a score that at least k codes reach: k / W of each wave's own maxima do.
-    const int each = (k + W - 1) / W;
-    const bool bounded = STAGED && k > 0 && each <= 64;
-    const float wmax = wave_max(own);
-    const uint32_t key = bounded ? lanes_above(key_of(own), each) : 0;
-    if ((tid & 63) == 0) {
-        s.redf[wave] = wmax;
-        s.redi[wave] = (int)key;
-    }
-    __syncthreads();
-    float mx = s.redf[0];
-    uint32_t low = (uint32_t)s.redi[0];
-#pragma unroll
-    for (int w = 1; w < W; ++w) {
-        mx = fmaxf(mx, s.redf[w]);
-        low = min(low, (uint32_t)s.redi[w]);
-    }
-    __syncthreads();
+    const bool bounded = HELD && k > 0 && k <= 64 * W;
+    float floor;
+    float mx = maximum<W>(own, k, bounded, s.redf, s.redi, &floor);
     if (mx == -INFINITY) {
         if (tid == 0) answer(-1, 0.f);
         return;
     }
-    float floor = low >= key_of(-INFINITY) ? score_of(low) : -INFINITY;
-    if (mx == INFINITY) {
-        mx = 0.f;
-        floor = -INFINITY;
-        if (STAGED) {
-            for (int c = tid; c < (V + 3) / 4 * 4; c += NT) lds[c] = S::narrow(S::widen(lds[c]) == INFINITY ? 0.f : -INFINITY);
-            __syncthreads();
-        } else {
-            row.inf = true;
-        }
-    }
-    Draw<DT, STAGED, W, L> d(s, row);
-    if (!(T > 0.0)) {                                               // the lowest index that has the maximum
-        int first = INT32_MAX;
-        d.each([&](float v, int c) { first = v == mx && c < first ? c : first; });
-        const float lowest = block_max_f32<W>(-(float)first, s.redf);  // indices are below 2^24
-        if (tid == 0) answer((int64_t)-lowest, 0.f);
+    if (!(T > 0.0)) {
+        const int first = first_of<DT, HELD, W>(mx, own, d.row, c0, c1, s.redf);
+        if (tid == 0) answer(first, 0.f);
         return;
     }
-    const Row r{(double)mx, fmin(1.0 / T, 1e300), ldexp(1.0, a.shift), mp > 1.0 ? 1.0 : mp};
-    // Where a bound says that the first cut lies among few codes, those become a list and one wave does the rest on it, without barriers; the
-    // others make room for the next row.
-    uint64_t Z = 0;
-    bool narrow = bounded;
-    if (STAGED && k <= 0 && P < 1.0) {
-        Z = d.total(d.sum([&](float v) { return r.units(v); }));
-        // The codes further than D from the maximum have at most V (exp(-D / T) 2^shift + 1) units.  That much may be missing of (1 - P) Z, less what
-        // rounding P Z and Z to f64 takes.
-        const double spare = (1.0 - P) * (double)Z * 0.999 - (double)V - 4096.0;
-        if (spare > 0.0) {
-            const double D = T * log((double)V * r.scale / spare);
-            narrow = D < 1e30;
-            floor = (float)((double)mx - fmax(D, 0.0) - fabs((double)mx) * 1e-6 - 1e-30);
+    if (mx == INFINITY) {                                           // the codes that have it share the draw
+        mx = 0.f;
+        floor = -INFINITY;
+        if (HELD) {
+            for (int c = d.from() + lane; c < c1; c += 64) lds[c] = S::narrow(S::widen(lds[c]) == INFINITY ? 0.f : -INFINITY);
+        } else {
+            d.row.inf = true;
         }
     }
-    if (STAGED && narrow) {
-        const int many = d.compact(floor);
-        if (many <= L::KEPT) {
-            if (wave) return;
-            Draw<DT, true, 1, L>(s, View<DT, true>{s.kept_x, many, false}).finish(r, mx, k, P, u, Z, [&](int c, float x, uint64_t mass) { answer(s.kept_i[c], a.logp ? r.logp(x, mass) : 0.f); });
+    const Row row(mx, T, a.min(n), a.shift);
+    uint64_t Z = 0;
+    if (k <= 0 && P < 1.0) {
+        Z = d.total(d.sum([&](float v) { return row.units(v); }));
+        // The codes further than D from the maximum have at most V (exp(-D / T) 2^shift + 1) units.  That much may be missing of (1 - P) Z, less
+        // what rounding P Z and Z to f64 takes.
+        const double spare = (1.0 - P) * (double)Z * 0.999 - (double)V - 4096.0;
+        if (spare > 0.0) {
+            const double D = T * log(ldexp((double)V, a.shift) / spare);
+            if (D < 1e30) floor = (float)((double)mx - fmax(D, 0.0) - fabs((double)mx) * 1e-6 - 1e-30);
+        }
+    }
+    if (HELD && few && floor > -INFINITY) {
+        const int many = d.compact(floor, *few);
+        together<W>();
+        if (many <= KEPT) {                                         // one wave does the rest, without barriers; the others make room
+            if (W > 1 && tid >= 64) return;
+            Draw<DT, true, 1, H::BINS> l(s.search, s.red, s.counts, View<DT, true>{few->x, many, false});
+            l.finish(row, mx, k, P, a.u[n], Z, [&](int c, float x, uint64_t mass) { answer(few->i[c], a.logp ? row.logp(x, mass) : 0.f); });
             return;
         }
     }
-    d.finish(r, mx, k, P, u, Z, [&](int c, float x, uint64_t mass) { answer(c, a.logp ? r.logp(x, mass) : 0.f); });
+    d.from_score(floor);
+    d.finish(row, mx, k, P, a.u[n], Z, [&](int c, float x, uint64_t mass) { answer(c, a.logp ? row.logp(x, mass) : 0.f); });
+}
+template <int DT, bool HELD, int W>
+__global__ __launch_bounds__(64 * W, W == 8 ? 6 : W == 1 ? 5 : 4) void sample_kernel(const SampleArgs a)
+{
+    constexpr int KEPT = !HELD ? 4 : W == 1 ? 256 : 1024;
+    extern __shared__ __attribute__((aligned(16))) char staged[];
+    __shared__ Shared<W, W == 1 ? 128 : 256> s;
+    __shared__ Few<DT, KEPT> few;
+    draw_row<DT, HELD, W>(a, blockIdx.x, reinterpret_cast<typename Score<DT>::Raw *>(staged), s, &few);
+}
+
+// For many rows with top-k: a block takes W of them, one after the other as far as it needs the whole row - the next one is on its way
+// meanwhile - and what is done on a short list of codes is left to the end, where each wave has a row's.  Rows without such a list
+// come last, by the whole block.
+template <int DT, int W>
+__global__ __launch_bounds__(64 * W, W == 8 ? 6 : 4) void sample_many_kernel(const SampleArgs a)
+{
+    typedef Score<DT> S;
+    constexpr int KEPT = 256, QUADS = 4, LISTED = 128;              // LISTED: bins for a list's cuts
+    typedef Few<DT, KEPT> F;
+    extern __shared__ __attribute__((aligned(16))) char staged[];
+    __shared__ Shared<W, 256> s;
+    __shared__ F few[W];
+    const int V = a.V, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const int64_t n0 = (int64_t)blockIdx.x * W;
+    const int rows = (int)min((int64_t)W, a.rows - n0);
+    typename S::Raw *lds = reinterpret_cast<typename S::Raw *>(staged);
+    const auto answer = [&](int r, int64_t i, float lp) {
+        a.idx[n0 + r] = i;
+        if (a.logp) a.logp[n0 + r] = lp;
+    };
+    if (tid < rows) {
+        F &f = few[tid];
+        f.T = a.T(n0 + tid);
+        f.P = a.P(n0 + tid);
+        f.min_p = a.min(n0 + tid);
+        f.k = a.k(n0 + tid);
+        f.u = a.u[n0 + tid];
+        f.padded = a.padded && a.padded[n0 + tid];
+        f.state = F::DONE;
+    }
+    Draw<DT, true, W, 256> d(s.search, s.red, s.counts, View<DT, true>{lds, V, false});
+    const int c0 = d.from() + lane * 4, c1 = d.to();                // a lane has at most QUADS quads
+    typename S::Raw4 raw[QUADS];
+    const auto load = [&](int r) {
+        const typename S::Raw *z = reinterpret_cast<const typename S::Raw *>(a.z) + (n0 + r) * a.ld;
+#pragma unroll
+        for (int q = 0; q < QUADS; ++q) {
+            const int c = c0 + q * 256;
+            if (c + 4 <= c1) {
+                raw[q] = *reinterpret_cast<const typename S::Raw4 *>(z + c);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) raw[q][i] = c + i < c1 ? z[c + i] : S::narrow(-INFINITY);
+            }
+        }
+    };
+    load(0);
+    __syncthreads();
+#pragma unroll 1
+    for (int r = 0; r < rows; ++r) {
+        const int k = few[r].k;
+        const bool greedy = !(few[r].T > 0.0), padded = few[r].padded, bounded = k > 0 && k <= 64 * W && !greedy;
+        float own = -INFINITY;                                      // the thread's maximum
+#pragma unroll
+        for (int q = 0; q < QUADS; ++q) {                           // each wave reads what it wrote itself: no barrier
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = clean(S::widen(raw[q][i]));
+                own = fmaxf(own, x[i]);
+            }
+            if (c0 + q * 256 < c1)
+                *reinterpret_cast<typename S::Quad *>(lds + c0 + q * 256) = typename S::Quad{S::narrow(x[0]), S::narrow(x[1]), S::narrow(x[2]), S::narrow(x[3])};
+        }
+        if (r + 1 < rows && !few[r + 1].padded) load(r + 1);
+        float floor;
+        const float mx = maximum<W>(own, k, bounded, s.redf, s.redi, &floor);
+        int state = F::DONE;
+        if (padded || mx == -INFINITY) {
+            if (tid == 0) answer(r, -1, 0.f);
+        } else if (greedy) {
+            const int first = first_of<DT, true, W>(mx, own, d.row, c0, c1, s.redf);
+            if (tid == 0) answer(r, first, 0.f);
+        } else {
+            state = F::WHOLE;
+            if (bounded && floor > -INFINITY && mx < INFINITY) {
+                const int many = d.compact(floor, few[r]);
+                if (many <= KEPT) state = many;
+            }
+        }
+        if (tid == 0) {
+            few[r].max = mx;
+            few[r].state = state;
+        }
+        __syncthreads();
+    }
+    if (wave < rows && few[wave].state >= 0) {
+        const F &f = few[wave];
+        const Row row(f.max, f.T, f.min_p, a.shift);
+        Search<LISTED> &there = reinterpret_cast<Search<LISTED> *>(staged)[wave];      // in the place of the rows
+        Draw<DT, true, 1, LISTED> l(there, s.red + wave, s.counts + wave, View<DT, true>{f.x, f.state, false});
+        l.finish(row, f.max, f.k, f.P, f.u, 0, [&](int c, float x, uint64_t mass) { answer(wave, f.i[c], a.logp ? row.logp(x, mass) : 0.f); });
+    }
+#pragma unroll 1
+    for (int r = 0; r < rows; ++r) {
+        if (few[r].state != F::WHOLE) continue;
+        __syncthreads();
+        draw_row<DT, true, W>(a, n0 + r, lds, s, (F *)nullptr);
+    }
 }
 
 }  // namespace mq
@@ -684,21 +848,35 @@ using namespace mq;
 
 // Waves a row: with many rows as few as keep a compute unit's 32 waves busy next to the rows' LDS, with too few rows to fill the chip as many
 // as the row has quads for, up to 16.
-template <int DT>
-static void sample_launch(const SampleArgs &a, int64_t rows, hipStream_t s)
+template <int DT, int W>
+static void sample_go(const SampleArgs &a, bool many, hipStream_t s)
 {
-    const dim3 grid((unsigned)rows);
     const size_t bytes = ((size_t)a.V + 3) / 4 * 4 * sizeof(typename Score<DT>::Raw);
-#define GO(W) hipLaunchKernelGGL((sample_kernel<DT, true, W>), grid, dim3(64 * W), bytes, s, a)
-    if (bytes > 48 * 1024) hipLaunchKernelGGL((sample_kernel<DT, false, 8>), grid, dim3(512), 0, s, a);
-    else if (rows < 256) {
-        if (a.V <= 1024) GO(4);
-        else if (a.V <= 2048) GO(8);
-        else GO(16);
-    } else if (a.V <= 1024) GO(2);
-    else if (a.V <= 4096) GO(4);
-    else GO(8);
-#undef GO
+    if constexpr (W == 4 || W == 8) {
+        if (many) {
+            hipLaunchKernelGGL((sample_many_kernel<DT, W>), dim3((unsigned)((a.rows + W - 1) / W)), dim3(64 * W), std::max(bytes, W * sizeof(Search<128>)), s, a);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((sample_kernel<DT, true, W>), dim3((unsigned)a.rows), dim3(64 * W), bytes, s, a);
+}
+template <int DT>
+static void sample_launch(const SampleArgs &a, hipStream_t s)
+{
+    const bool k = a.top_k || (a.k0 > 0 && a.k0 < a.V);
+    if (a.V > 16384) hipLaunchKernelGGL((sample_kernel<DT, false, 8>), dim3((unsigned)a.rows), dim3(512), 0, s, a);
+    else if (a.rows < 256) {
+        if (a.V <= 1024) sample_go<DT, 4>(a, false, s);
+        else sample_go<DT, 16>(a, false, s);
+    } else if (a.V <= 1024) {
+        sample_go<DT, 1>(a, false, s);
+    } else if (a.V <= 4096) {
+        sample_go<DT, 4>(a, k, s);
+    } else if (a.V <= 8192) {
+        sample_go<DT, 8>(a, k, s);
+    } else {
+        sample_go<DT, 16>(a, false, s);
+    }
 }
 
 extern "C" int mq_sample_codes(const mqSampleDesc *d, const void *logits, const float *uniform, const float *temperature, const int32_t *top_k,
@@ -715,10 +893,10 @@ extern "C" int mq_sample_codes(const mqSampleDesc *d, const void *logits, const 
     int bits = 0;
     while ((1ll << bits) < d->codes) ++bits;
     const int shift = 62 - bits < 51 ? 62 - bits : 51;
-    const SampleArgs a{logits, d->row_stride, d->codes, shift, uniform, temperature, top_p, min_p, top_k, d->temperature, d->top_p, d->min_p, d->top_k, padded, idx, logp};
-    if (d->dtype == 0) sample_launch<0>(a, d->rows, S(stream));
-    else if (d->dtype == 1) sample_launch<1>(a, d->rows, S(stream));
-    else sample_launch<2>(a, d->rows, S(stream));
+    const SampleArgs a{logits, d->row_stride, d->codes, shift, uniform, temperature, top_p, min_p, top_k, d->temperature, d->top_p, d->min_p, d->top_k, padded, idx, logp, d->rows};
+    if (d->dtype == 0) sample_launch<0>(a, S(stream));
+    else if (d->dtype == 1) sample_launch<1>(a, S(stream));
+    else sample_launch<2>(a, S(stream));
     MQ_LAUNCH_CHECK("mq_sample_codes");
     return 0;
 }
