@@ -39,6 +39,7 @@ struct SampleArgs {
     int64_t *idx;
     float *logp;
     int64_t rows;
+    int squeezes;                                                    // the rows' LDS has room for V indices
     __device__ __forceinline__ double T(int64_t n) const { return temperature ? (double)temperature[n] : t0; }
     __device__ __forceinline__ double P(int64_t n) const { return top_p ? (double)top_p[n] : p0; }
     __device__ __forceinline__ double min(int64_t n) const { return min_p ? (double)min_p[n] : m0; }
@@ -203,23 +204,24 @@ template <int W> __device__ __forceinline__ void together();
 template <int BINS, bool FROM_TOP, int W, typename U>
 __device__ __forceinline__ void find_bin(const U *hist, uint64_t goal, Found *out)
 {
-    if (threadIdx.x < 64) {
+    const int lane = W > 1 ? (int)threadIdx.x : (int)threadIdx.x & 63;
+    if (lane < 64) {
         constexpr int PER = BINS / 64;
         uint64_t mine = 0;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) mine += hist[FROM_TOP ? BINS - 1 - ((int)threadIdx.x * PER + i) : (int)threadIdx.x * PER + i];
+        for (int i = 0; i < PER; ++i) mine += hist[FROM_TOP ? BINS - 1 - (lane * PER + i) : lane * PER + i];
         const uint64_t upto = wave_scan(mine);
-        if (threadIdx.x == 63) out->total = upto;
+        if (lane == 63) out->total = upto;
         if (upto >= goal && upto - mine < goal) {
             uint64_t before = upto - mine;
             int i = 0;
             for (; i < PER - 1; ++i) {
-                const uint64_t h = hist[FROM_TOP ? BINS - 1 - ((int)threadIdx.x * PER + i) : (int)threadIdx.x * PER + i];
+                const uint64_t h = hist[FROM_TOP ? BINS - 1 - (lane * PER + i) : lane * PER + i];
                 if (before + h >= goal) break;
                 before += h;
             }
             out->before = before;
-            out->bin = FROM_TOP ? BINS - 1 - ((int)threadIdx.x * PER + i) : (int)threadIdx.x * PER + i;
+            out->bin = FROM_TOP ? BINS - 1 - (lane * PER + i) : lane * PER + i;
         }
     }
     together<W>();
@@ -258,7 +260,7 @@ struct Entry {
 // What a cut is found with
 template <int NBINS>
 struct Search {
-    static constexpr int BINS = NBINS, LIST = NBINS / 2;
+    static constexpr int BINS = NBINS, LIST = NBINS / 4;
     unsigned long long hist[BINS];
     Entry list[LIST];                                               // codes of the bin that a cut falls into
     float cut_x;
@@ -308,13 +310,16 @@ struct Draw {
     View<DT, STAGED> row;
     float cut_x;                                                    // kept: at or before (cut_x, cut_i) in the order
     int cut_i;
+    int begin, end;
 
-    __device__ __forceinline__ Draw(Search<BINS> &s_, unsigned long long *red_, int *redi_, const View<DT, STAGED> &v) : s(s_), red(red_), redi(redi_), row(v), cut_x(-INFINITY), cut_i(-1) {}      // nothing with a score of -inf
-    // The wave's part of the row: codes [from, to), a multiple of 256 from the last one's
+    __device__ __forceinline__ Draw(Search<BINS> &s_, unsigned long long *red_, int *redi_, const View<DT, STAGED> &v) : s(s_), red(red_), redi(redi_), row(v), cut_x(-INFINITY), cut_i(-1)
+    {                                                               // nothing with a score of -inf
+        const int part = (row.n + 256 * W - 1) / (256 * W) * 256;
+        begin = wave() * part;
+        end = min(begin + part, row.n);
+    }
+    // The wave's part of the row: codes [begin, end), a multiple of 256 up to the last one's
     __device__ __forceinline__ int wave() const { return W > 1 ? (int)(threadIdx.x >> 6) : 0; }
-    __device__ __forceinline__ int part() const { return (row.n + 256 * W - 1) / (256 * W) * 256; }
-    __device__ __forceinline__ int from() const { return wave() * part(); }
-    __device__ __forceinline__ int to() const { return min(from() + part(), row.n); }
     __device__ __forceinline__ bool kept(float x, int c) const { return x > cut_x || (x == cut_x && c <= cut_i); }
     // all codes with scores from x up may be kept
     __device__ __forceinline__ void from_score(float x)
@@ -326,9 +331,9 @@ struct Draw {
     template <typename F>
     __device__ __forceinline__ void each(F f) const
     {
-        const int c1 = to();
+        const int c1 = end;
 #pragma unroll 1
-        for (int c = from() + (threadIdx.x & 63); c < c1; c += 64) {
+        for (int c = begin + (threadIdx.x & 63); c < c1; c += 64) {
             const float x = row.one(c);
             if (kept(x, c)) f(x, c);
         }
@@ -338,9 +343,9 @@ struct Draw {
     __device__ __forceinline__ uint64_t sum(Q q) const
     {
         uint64_t t = 0;
-        const int c1 = to();
+        const int c1 = end;
 #pragma unroll 1
-        for (int c = from() + (threadIdx.x & 63) * 4; c < c1; c += 256) {
+        for (int c = begin + (threadIdx.x & 63) * 4; c < c1; c += 256) {
             float x[4];
             row.four(c, x);
             bool in[4], any = false;
@@ -380,7 +385,7 @@ struct Draw {
         const float border = score_of((uint32_t)prefix);
         const uint64_t w = q(border);
         const int need = (int)((goal - above + w - 1) / w);
-        const int lane = threadIdx.x & 63, c0 = from(), c1 = to();
+        const int lane = threadIdx.x & 63, c0 = begin, c1 = end;
         uint32_t mine = 0;
         each([&](float v, int) { mine += v == border; });
         const int count = (int)wave_total(mine);
@@ -512,9 +517,9 @@ struct Draw {
             }
         }
         if (wave() != mine) return;
-        const int c1 = to();
+        const int c1 = end;
 #pragma unroll 1
-        for (int c = from(); c < c1; c += 256) {                    // the wave's lanes go round together
+        for (int c = begin; c < c1; c += 256) {                    // the wave's lanes go round together
             float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             const int at = c + lane * 4;
             if (at < c1) row.four(at, x);
@@ -557,7 +562,7 @@ struct Draw {
     template <int KEPT>
     __device__ __forceinline__ int compact(float floor, Few<DT, KEPT> &few)
     {
-        const int lane = threadIdx.x & 63, c0 = from(), c1 = to();
+        const int lane = threadIdx.x & 63, c0 = begin, c1 = end;
         const auto in = [&](float v) { return v >= floor && v > -INFINITY; };
         int count = 0;
 #pragma unroll 1
@@ -598,27 +603,69 @@ struct Draw {
         }
         return many;
     }
+    // Leaves the codes with x >= floor only, each wave in its part of the row: packed in index order, index[place] the code.  How many a wave's are.
+    __device__ __forceinline__ int squeeze(typename Score<DT>::Raw *x_, uint16_t *index, float floor)
+    {
+        const int lane = threadIdx.x & 63;
+        const auto in = [&](float v) { return v >= floor && v > -INFINITY; };
+        int at = begin;
+#pragma unroll 1
+        for (int c = begin; c < end; c += 256) {                    // all lanes go round together; they write at or before what they have read
+            float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (c + lane * 4 < end) row.four(c + lane * 4, x);
+            together<1>();
+            int place = at;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint64_t m = __builtin_amdgcn_ballot_w64(in(x[i]));
+                place += (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
+                at += __popcll(m);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (in(x[i])) {
+                    x_[place] = Score<DT>::narrow(x[i]);
+                    index[place++] = (uint16_t)(c + lane * 4 + i);
+                }
+        }
+        if (lane < (-at & 3)) x_[at + lane] = Score<DT>::narrow(-INFINITY);      // to whole quads
+        end = at;
+        together<1>();
+        return at - begin;
+    }
 };
 
-// The lower end (a score's key, its low 16 bits cleared) of what at least `need` of the wave's lanes have: bit by bit from the top.
-__device__ __forceinline__ uint32_t lanes_above(uint32_t key, int need)
+// The lower end (a score's key, its low 16 bits cleared) of what at least `need` of the wave's values have: bit by bit from the top.
+template <int G>
+__device__ __forceinline__ uint32_t values_above(const uint32_t (&key)[G], int need)
 {
     uint32_t t = 0;
 #pragma unroll
     for (int b = 31; b >= 16; --b) {
         const uint32_t with = t | 1u << b;
-        if (__popcll(__builtin_amdgcn_ballot_w64(key >= with)) >= need) t = with;
+        int many = 0;
+#pragma unroll
+        for (int g = 0; g < G; ++g) many += __popcll(__builtin_amdgcn_ballot_w64(key[g] >= with));
+        if (many >= need) t = with;
     }
     return t;
 }
 
-// The block's maximum, and a score that at least k codes reach where HELD and k <= 64 W: k / W of each wave's own maxima do.  own: the thread's.
-template <int W>
-__device__ __forceinline__ float maximum(float own, int k, bool bounded, float *redf, int *redi, float *floor)
+// The block's maximum, and a score that at least k codes reach where k <= 64 G W: k / W of each wave's own maxima do.  own: maxima of G groups
+// of the thread's codes.  Four groups cost 200 instructions more than one, so only a wave that has a whole row by itself takes them.
+template <int W, int G>
+__device__ __forceinline__ float maximum(const float (&own)[G], int k, float *redf, int *redi, float *floor)
 {
     const int wave = W > 1 ? threadIdx.x >> 6 : 0;
-    const float wmax = wave_max(own);
-    uint32_t low = bounded ? lanes_above(key_of(own), (k + W - 1) / W) : 0;
+    float most = own[0];
+    uint32_t key[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        most = fmaxf(most, own[g]);
+        key[g] = key_of(own[g]);
+    }
+    const float wmax = wave_max(most);
+    uint32_t low = k > 0 && k <= 64 * G * W ? values_above(key, (k + W - 1) / W) : 0;
     float mx = wmax;
     if (W > 1) {
         if ((threadIdx.x & 63) == 0) {
@@ -655,12 +702,13 @@ __device__ __forceinline__ int first_of(float mx, float own, const View<DT, STAG
     return (int)-block_max_f32<W>(-(float)first, redf);
 }
 
-// One row by a block of W waves.  HELD: it is read once, into LDS (at `lds`), each wave's part by itself; else each time from memory.  few: NULL,
-// or where a list of codes may go.
+// One row by a block of W waves.  HELD: it is read once, into LDS (at `lds`), each wave's part by itself; else each time from memory.  index:
+// NULL, or where V codes' indices may go, and few a list of the codes to keep.
 template <int DT, bool HELD, int W, typename H, int KEPT>
-__device__ __forceinline__ void draw_row(const SampleArgs &a, int64_t n, typename Score<DT>::Raw *lds, H &s, Few<DT, KEPT> *few)
+__device__ __forceinline__ void draw_row(const SampleArgs &a, int64_t n, typename Score<DT>::Raw *lds, H &s, uint16_t *index, Few<DT, KEPT> *few)
 {
     typedef Score<DT> S;
+    constexpr int G = W == 1 ? 4 : 1;
     const int V = a.V, tid = threadIdx.x, lane = tid & 63;
     const auto answer = [&](int64_t i, float lp) {
         a.idx[n] = i;
@@ -675,25 +723,32 @@ __device__ __forceinline__ void draw_row(const SampleArgs &a, int64_t n, typenam
     const typename S::Raw *z = reinterpret_cast<const typename S::Raw *>(a.z) + n * a.ld;
     Draw<DT, HELD, W, H::BINS> d(s.search, s.red, s.counts, View<DT, HELD>{HELD ? lds : z, V, false});
     const View<DT, false> from{z, V, false};
-    const int c0 = d.from() + lane * 4, c1 = d.to();
-    float own = -INFINITY;
-#pragma unroll 4
-    for (int c = c0; c < c1; c += 256) {
-        float x[4];
-        from.four(c, x);
+    const int c0 = d.begin + lane * 4, c1 = d.end;
+    float own[G], most = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) own = fmaxf(own, x[i]);
-        if (HELD) *reinterpret_cast<typename S::Quad *>(lds + c) = typename S::Quad{S::narrow(x[0]), S::narrow(x[1]), S::narrow(x[2]), S::narrow(x[3])};
+    for (int g = 0; g < G; ++g) own[g] = -INFINITY;
+    for (int c = c0; c < c1; c += 1024) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int at = c + q * 256;
+            if (at >= c1) continue;
+            float x[4];
+            from.four(at, x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) own[q % G] = fmaxf(own[q % G], x[i]);
+            if (HELD) *reinterpret_cast<typename S::Quad *>(lds + at) = typename S::Quad{S::narrow(x[0]), S::narrow(x[1]), S::narrow(x[2]), S::narrow(x[3])};
+        }
     }
-    const bool bounded = HELD && k > 0 && k <= 64 * W;
+#pragma unroll
+    for (int g = 0; g < G; ++g) most = fmaxf(most, own[g]);
     float floor;
-    float mx = maximum<W>(own, k, bounded, s.redf, s.redi, &floor);
+    float mx = maximum<W, G>(own, HELD ? k : 0, s.redf, s.redi, &floor);
     if (mx == -INFINITY) {
         if (tid == 0) answer(-1, 0.f);
         return;
     }
     if (!(T > 0.0)) {
-        const int first = first_of<DT, HELD, W>(mx, own, d.row, c0, c1, s.redf);
+        const int first = first_of<DT, HELD, W>(mx, most, d.row, c0, c1, s.redf);
         if (tid == 0) answer(first, 0.f);
         return;
     }
@@ -701,7 +756,7 @@ __device__ __forceinline__ void draw_row(const SampleArgs &a, int64_t n, typenam
         mx = 0.f;
         floor = -INFINITY;
         if (HELD) {
-            for (int c = d.from() + lane; c < c1; c += 64) lds[c] = S::narrow(S::widen(lds[c]) == INFINITY ? 0.f : -INFINITY);
+            for (int c = d.begin + lane; c < c1; c += 64) lds[c] = S::narrow(S::widen(lds[c]) == INFINITY ? 0.f : -INFINITY);
         } else {
             d.row.inf = true;
         }
@@ -718,27 +773,45 @@ __device__ __forceinline__ void draw_row(const SampleArgs &a, int64_t n, typenam
             if (D < 1e30) floor = (float)((double)mx - fmax(D, 0.0) - fabs((double)mx) * 1e-6 - 1e-30);
         }
     }
-    if (HELD && few && floor > -INFINITY) {
-        const int many = d.compact(floor, *few);
-        together<W>();
-        if (many <= KEPT) {                                         // one wave does the rest, without barriers; the others make room
-            if (W > 1 && tid >= 64) return;
-            Draw<DT, true, 1, H::BINS> l(s.search, s.red, s.counts, View<DT, true>{few->x, many, false});
-            l.finish(row, mx, k, P, a.u[n], Z, [&](int c, float x, uint64_t mass) { answer(few->i[c], a.logp ? row.logp(x, mass) : 0.f); });
-            return;
+    const bool squeezed = HELD && index && floor > -INFINITY;
+    if (squeezed) {
+        const int count = d.squeeze(lds, index, floor);
+        if (W > 1) {
+            if (lane == 0) s.counts[tid >> 6] = count;
+            __syncthreads();
+            int at = 0, many = 0;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                at += w < tid >> 6 ? s.counts[w] : 0;
+                many += s.counts[w];
+            }
+            if (many <= KEPT) {                                     // one wave does the rest, without barriers; the others make room
+                for (int c = lane; c < count; c += 64) {
+                    few->x[at + c] = lds[d.begin + c];
+                    few->i[at + c] = index[d.begin + c];
+                }
+                if (tid < (-many & 3)) few->x[many + tid] = S::narrow(-INFINITY);
+                __syncthreads();
+                if (tid >= 64) return;
+                Draw<DT, true, 1, H::BINS> l(s.search, s.red, s.counts, View<DT, true>{few->x, many, false});
+                l.finish(row, mx, k, P, a.u[n], Z, [&](int c, float x, uint64_t mass) { answer(few->i[c], a.logp ? row.logp(x, mass) : 0.f); });
+                return;
+            }
         }
     }
     d.from_score(floor);
-    d.finish(row, mx, k, P, a.u[n], Z, [&](int c, float x, uint64_t mass) { answer(c, a.logp ? row.logp(x, mass) : 0.f); });
+    d.finish(row, mx, k, P, a.u[n], Z, [&](int c, float x, uint64_t mass) { answer(squeezed ? index[c] : c, a.logp ? row.logp(x, mass) : 0.f); });
 }
 template <int DT, bool HELD, int W>
 __global__ __launch_bounds__(64 * W, W == 8 ? 6 : W == 1 ? 5 : 4) void sample_kernel(const SampleArgs a)
 {
-    constexpr int KEPT = !HELD ? 4 : W == 1 ? 256 : 1024;
+    constexpr int KEPT = !HELD || W == 1 ? 4 : 192;                 // a whole row's wave needs no list beside it; three rows of 8192 to a compute unit
+    typedef typename Score<DT>::Raw Raw;
     extern __shared__ __attribute__((aligned(16))) char staged[];
     __shared__ Shared<W, W == 1 ? 128 : 256> s;
     __shared__ Few<DT, KEPT> few;
-    draw_row<DT, HELD, W>(a, blockIdx.x, reinterpret_cast<typename Score<DT>::Raw *>(staged), s, &few);
+    Raw *lds = reinterpret_cast<Raw *>(staged);
+    draw_row<DT, HELD, W>(a, blockIdx.x, lds, s, a.squeezes ? reinterpret_cast<uint16_t *>(lds + (a.V + 3) / 4 * 4) : nullptr, &few);
 }
 
 // For many rows with top-k: a block takes W of them, one after the other as far as it needs the whole row - the next one is on its way
@@ -772,7 +845,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 6 : 4) void sample_many_kernel(con
         f.state = F::DONE;
     }
     Draw<DT, true, W, 256> d(s.search, s.red, s.counts, View<DT, true>{lds, V, false});
-    const int c0 = d.from() + lane * 4, c1 = d.to();                // a lane has at most QUADS quads
+    const int c0 = d.begin + lane * 4, c1 = d.end;                // a lane has at most QUADS quads
     typename S::Raw4 raw[QUADS];
     const auto load = [&](int r) {
         const typename S::Raw *z = reinterpret_cast<const typename S::Raw *>(a.z) + (n0 + r) * a.ld;
@@ -792,31 +865,31 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 6 : 4) void sample_many_kernel(con
 #pragma unroll 1
     for (int r = 0; r < rows; ++r) {
         const int k = few[r].k;
-        const bool greedy = !(few[r].T > 0.0), padded = few[r].padded, bounded = k > 0 && k <= 64 * W && !greedy;
-        float own = -INFINITY;                                      // the thread's maximum
+        const bool greedy = !(few[r].T > 0.0), padded = few[r].padded;
+        float own[1] = {-INFINITY};                                 // the thread's maximum
 #pragma unroll
         for (int q = 0; q < QUADS; ++q) {                           // each wave reads what it wrote itself: no barrier
             float x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 x[i] = clean(S::widen(raw[q][i]));
-                own = fmaxf(own, x[i]);
+                own[0] = fmaxf(own[0], x[i]);
             }
             if (c0 + q * 256 < c1)
                 *reinterpret_cast<typename S::Quad *>(lds + c0 + q * 256) = typename S::Quad{S::narrow(x[0]), S::narrow(x[1]), S::narrow(x[2]), S::narrow(x[3])};
         }
         if (r + 1 < rows && !few[r + 1].padded) load(r + 1);
         float floor;
-        const float mx = maximum<W>(own, k, bounded, s.redf, s.redi, &floor);
+        const float mx = maximum<W, 1>(own, greedy ? 0 : k, s.redf, s.redi, &floor);
         int state = F::DONE;
         if (padded || mx == -INFINITY) {
             if (tid == 0) answer(r, -1, 0.f);
         } else if (greedy) {
-            const int first = first_of<DT, true, W>(mx, own, d.row, c0, c1, s.redf);
+            const int first = first_of<DT, true, W>(mx, own[0], d.row, c0, c1, s.redf);
             if (tid == 0) answer(r, first, 0.f);
         } else {
             state = F::WHOLE;
-            if (bounded && floor > -INFINITY && mx < INFINITY) {
+            if (floor > -INFINITY && mx < INFINITY) {
                 const int many = d.compact(floor, few[r]);
                 if (many <= KEPT) state = many;
             }
@@ -838,7 +911,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 6 : 4) void sample_many_kernel(con
     for (int r = 0; r < rows; ++r) {
         if (few[r].state != F::WHOLE) continue;
         __syncthreads();
-        draw_row<DT, true, W>(a, n0 + r, lds, s, (F *)nullptr);
+        draw_row<DT, true, W>(a, n0 + r, lds, s, nullptr, (F *)nullptr);
     }
 }
 
@@ -848,35 +921,31 @@ using namespace mq;
 
 // Waves a row: with many rows as few as keep a compute unit's 32 waves busy next to the rows' LDS, with too few rows to fill the chip as many
 // as the row has quads for, up to 16.
+constexpr size_t ROOM = 58 * 1024;       // for a row and its indices: LDS that needs no leave from the runtime, less the kernels' own
+template <int DT>
+static size_t row_bytes(int V) { return ((size_t)V + 3) / 4 * 4 * sizeof(typename Score<DT>::Raw); }
 template <int DT, int W>
-static void sample_go(const SampleArgs &a, bool many, hipStream_t s)
+static void sample_go(SampleArgs a, hipStream_t s)
 {
-    const size_t bytes = ((size_t)a.V + 3) / 4 * 4 * sizeof(typename Score<DT>::Raw);
-    if constexpr (W == 4 || W == 8) {
-        if (many) {
-            hipLaunchKernelGGL((sample_many_kernel<DT, W>), dim3((unsigned)((a.rows + W - 1) / W)), dim3(64 * W), std::max(bytes, W * sizeof(Search<128>)), s, a);
-            return;
-        }
-    }
-    hipLaunchKernelGGL((sample_kernel<DT, true, W>), dim3((unsigned)a.rows), dim3(64 * W), bytes, s, a);
+    const size_t row = row_bytes<DT>(a.V), index = (size_t)a.V * sizeof(uint16_t);
+    a.squeezes = row + index <= ROOM && (a.top_k || a.k0 > 0 || a.top_p || a.p0 < 1.0);
+    hipLaunchKernelGGL((sample_kernel<DT, true, W>), dim3((unsigned)a.rows), dim3(64 * W), row + (a.squeezes ? index : 0), s, a);
+}
+template <int DT, int W>
+static void sample_many(const SampleArgs &a, hipStream_t s)
+{
+    hipLaunchKernelGGL((sample_many_kernel<DT, W>), dim3((unsigned)((a.rows + W - 1) / W)), dim3(64 * W), std::max(row_bytes<DT>(a.V), W * sizeof(Search<128>)), s, a);
 }
 template <int DT>
 static void sample_launch(const SampleArgs &a, hipStream_t s)
 {
-    const bool k = a.top_k || (a.k0 > 0 && a.k0 < a.V);
-    if (a.V > 16384) hipLaunchKernelGGL((sample_kernel<DT, false, 8>), dim3((unsigned)a.rows), dim3(512), 0, s, a);
-    else if (a.rows < 256) {
-        if (a.V <= 1024) sample_go<DT, 4>(a, false, s);
-        else sample_go<DT, 16>(a, false, s);
-    } else if (a.V <= 1024) {
-        sample_go<DT, 1>(a, false, s);
-    } else if (a.V <= 4096) {
-        sample_go<DT, 4>(a, k, s);
-    } else if (a.V <= 8192) {
-        sample_go<DT, 8>(a, k, s);
-    } else {
-        sample_go<DT, 16>(a, false, s);
-    }
+    const bool list = a.top_k || (a.k0 > 0 && a.k0 <= 128) || (!a.temperature && a.t0 == 0.0);
+    if (a.V > 16384 || row_bytes<DT>(a.V) > ROOM) hipLaunchKernelGGL((sample_kernel<DT, false, 8>), dim3((unsigned)a.rows), dim3(512), 0, s, a);
+    else if (a.rows < 256 && a.V <= 1024) sample_go<DT, 4>(a, s);
+    else if (a.rows < 256 || a.V > 8192) sample_go<DT, 16>(a, s);
+    else if (a.V <= 1024) sample_go<DT, 1>(a, s);
+    else if (a.V <= 4096) list ? sample_many<DT, 4>(a, s) : sample_go<DT, 4>(a, s);
+    else list ? sample_many<DT, 8>(a, s) : sample_go<DT, 8>(a, s);
 }
 
 extern "C" int mq_sample_codes(const mqSampleDesc *d, const void *logits, const float *uniform, const float *temperature, const int32_t *top_k,
@@ -893,7 +962,7 @@ extern "C" int mq_sample_codes(const mqSampleDesc *d, const void *logits, const 
     int bits = 0;
     while ((1ll << bits) < d->codes) ++bits;
     const int shift = 62 - bits < 51 ? 62 - bits : 51;
-    const SampleArgs a{logits, d->row_stride, d->codes, shift, uniform, temperature, top_p, min_p, top_k, d->temperature, d->top_p, d->min_p, d->top_k, padded, idx, logp, d->rows};
+    const SampleArgs a{logits, d->row_stride, d->codes, shift, uniform, temperature, top_p, min_p, top_k, d->temperature, d->top_p, d->min_p, d->top_k, padded, idx, logp, d->rows, 0};
     if (d->dtype == 0) sample_launch<0>(a, S(stream));
     else if (d->dtype == 1) sample_launch<1>(a, S(stream));
     else sample_launch<2>(a, S(stream));
