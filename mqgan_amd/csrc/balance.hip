@@ -623,7 +623,7 @@ extern "C" size_t mq_code_balance_workspace(int64_t rows, int codes, int dtype)
     else if (f.tl == 8) F(8, 1, 1);                                       \
     else if (f.tl == 16) F(16, 1, 1);                                     \
     else if (f.tl == 32) F(32, 1, 1);                                     \
-    else if (f.w == 16) F(64, 4, 16);                                     \
+    else if (f.w == 16) { if constexpr (sizeof(T) == 4) F(64, 4, 16); }   \
     else if (f.w == 8 && f.nq == 4) F(64, 4, 8);                          \
     else if (f.w == 8) F(64, 2, 8);                                       \
     else if (f.w == 4) F(64, 2, 4);                                       \

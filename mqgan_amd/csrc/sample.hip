@@ -128,6 +128,13 @@ __device__ __forceinline__ double exp2_half(double r)
     q = fma(q, r, 6.931471805599453e-01);
     return fma(q, r, 1.0);
 }
+// ln x, 1 <= x < 2^64, to 1e-13: the f32 instruction's log2, corrected by how far 2 to its power is from x
+__device__ __forceinline__ double ln(double x)
+{
+    const double y = (double)__builtin_amdgcn_logf((float)x), n = rint(y);
+    const double off = ldexp(x * exp2_half(n - y), -(int)n) - 1.0;  // about 1e-6 at most
+    return fma(y, 0.6931471805599453, off * fma(off, -0.5, 1.0));
+}
 // What of a row's settings the weights need; max is finite (rows with +inf are remapped to scores 0 and -inf before)
 struct Row {
     double max, per_t;                   // 1 / T; 0 for T = inf
@@ -148,7 +155,7 @@ struct Row {
         return d < -1074.8 || w < limit ? 0 : q;
     }
     // log of a weight's share of Z units
-    __device__ __forceinline__ float logp(float x, uint64_t Z) const { return (float)(((double)x - max) * per_t - log(ldexp((double)Z, -shift))); }
+    __device__ __forceinline__ float logp(float x, uint64_t Z) const { return (float)(((double)x - max) * per_t - ln(ldexp((double)Z, -shift))); }
 };
 
 // Inclusive scans over the 64 lanes by DPP (row shifts, then the rows' last lanes broadcast): a tenth of the latency of the LDS crossbar's.
@@ -769,7 +776,7 @@ __device__ __forceinline__ void draw_row(const SampleArgs &a, int64_t n, typenam
         // what rounding P Z and Z to f64 takes.
         const double spare = (1.0 - P) * (double)Z * 0.999 - (double)V - 4096.0;
         if (spare > 0.0) {
-            const double D = T * log(ldexp((double)V, a.shift) / spare);
+            const double D = T * ln(fmax(ldexp((double)V, a.shift) / spare, 1.0));
             if (D < 1e30) floor = (float)((double)mx - fmax(D, 0.0) - fabs((double)mx) * 1e-6 - 1e-30);
         }
     }
@@ -911,7 +918,9 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 6 : 4) void sample_many_kernel(con
     for (int r = 0; r < rows; ++r) {
         if (few[r].state != F::WHOLE) continue;
         __syncthreads();
-        draw_row<DT, true, W>(a, n0 + r, lds, s, nullptr, (F *)nullptr);
+        SampleArgs b = a;
+        asm volatile("" : "+s"(b.V));                               // nothing of the body is worked out before the loop: it would be spilled
+        draw_row<DT, true, W>(b, n0 + r, lds, s, nullptr, (F *)nullptr);
     }
 }
 
