@@ -565,19 +565,24 @@ struct Draw {
         const double g = ceil(P * (double)Z);
         return g > 1.0 ? (uint64_t)g : 1;
     }
-    // Puts the codes with x >= floor into the list of kept codes, in index order, where they are at most KEPT.  How many they are.
-    template <int KEPT>
+    // Puts the codes with x >= floor (> -inf) into the list of kept codes, in index order, where they are at most KEPT.  How many they are.  For
+    // parts of at most 64 SLOTS codes: one comparison a code, and where none of 64 is kept nothing else.
+    template <int SLOTS, int KEPT>
     __device__ __forceinline__ int compact(float floor, Few<DT, KEPT> &few)
     {
-        const int lane = threadIdx.x & 63, c0 = begin, c1 = end;
-        const auto in = [&](float v) { return v >= floor && v > -INFINITY; };
-        int count = 0;
-#pragma unroll 1
-        for (int c = c0; c < c1; c += 256) {                        // all lanes of a wave go round together
-            float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            if (c + lane * 4 < c1) row.four(c + lane * 4, x);
+        const int lane = threadIdx.x & 63;
+        float x[SLOTS];
+        uint64_t m[SLOTS];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) count += __popcll(__builtin_amdgcn_ballot_w64(in(x[i])));
+        for (int j = 0; j < SLOTS; ++j) {
+            const int c = begin + j * 64 + lane;
+            x[j] = c < end ? row.one(c) : (float)-INFINITY;
+        }
+        int count = 0;
+#pragma unroll
+        for (int j = 0; j < SLOTS; ++j) {
+            m[j] = __builtin_amdgcn_ballot_w64(x[j] >= floor);
+            count += __popcll(m[j]);
         }
         if (lane == 0) redi[wave()] = count;
         together<W>();
@@ -588,52 +593,44 @@ struct Draw {
             many += redi[w];
         }
         if (many <= KEPT) {
-#pragma unroll 1
-            for (int c = c0; c < c1 && count; c += 256) {
-                float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                if (c + lane * 4 < c1) row.four(c + lane * 4, x);
-                int place = at;
+            at = __builtin_amdgcn_readfirstlane(at);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint64_t m = __builtin_amdgcn_ballot_w64(in(x[i]));
-                    place += (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
-                    at += __popcll(m);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (in(x[i])) {
-                        few.x[place] = Score<DT>::narrow(x[i]);
-                        few.i[place++] = (uint16_t)(c + lane * 4 + i);
+            for (int j = 0; j < SLOTS; ++j) {
+                if (m[j]) {                                          // the same in all lanes
+                    const int place = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m[j], (uint32_t)at));
+                    if (x[j] >= floor) {
+                        few.x[place] = Score<DT>::narrow(x[j]);
+                        few.i[place] = (uint16_t)(begin + j * 64 + lane);
                     }
+                    at += __popcll(m[j]);
+                }
             }
             if (threadIdx.x < (unsigned)(-many & 3)) few.x[many + threadIdx.x] = Score<DT>::narrow(-INFINITY);      // to whole quads
         }
         return many;
     }
-    // Leaves the codes with x >= floor only, each wave in its part of the row: packed in index order, index[place] the code.  How many a wave's are.
+    // Leaves the codes with x >= floor (> -inf) only, each wave in its part of the row: packed in index order, index[place] the code.  How many a
+    // wave's are.
     __device__ __forceinline__ int squeeze(typename Score<DT>::Raw *x_, uint16_t *index, float floor)
     {
         const int lane = threadIdx.x & 63;
-        const auto in = [&](float v) { return v >= floor && v > -INFINITY; };
         int at = begin;
 #pragma unroll 1
-        for (int c = begin; c < end; c += 256) {                    // all lanes go round together; they write at or before what they have read
-            float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            if (c + lane * 4 < end) row.four(c + lane * 4, x);
-            together<1>();
-            int place = at;
+        for (int c = begin + lane; c < begin + (end - begin + 255) / 256 * 256; c += 256) {      // all lanes go round together
+            float x[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint64_t m = __builtin_amdgcn_ballot_w64(in(x[i]));
-                place += (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
+            for (int j = 0; j < 4; ++j) x[j] = c + j * 64 < end ? row.one(c + j * 64) : (float)-INFINITY;
+            together<1>();                                           // they write at or before what they have read
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint64_t m = __builtin_amdgcn_ballot_w64(x[j] >= floor);
+                const int place = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, (uint32_t)at));
+                if (x[j] >= floor) {
+                    x_[place] = Score<DT>::narrow(x[j]);
+                    index[place] = (uint16_t)(c + j * 64);
+                }
                 at += __popcll(m);
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (in(x[i])) {
-                    x_[place] = Score<DT>::narrow(x[i]);
-                    index[place++] = (uint16_t)(c + lane * 4 + i);
-                }
         }
         if (lane < (-at & 3)) x_[at + lane] = Score<DT>::narrow(-INFINITY);      // to whole quads
         end = at;
@@ -897,7 +894,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 6 : 4) void sample_many_kernel(con
         } else {
             state = F::WHOLE;
             if (floor > -INFINITY && mx < INFINITY) {
-                const int many = d.compact(floor, few[r]);
+                const int many = d.template compact<4 * QUADS>(floor, few[r]);
                 if (many <= KEPT) state = many;
             }
         }

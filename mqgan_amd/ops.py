@@ -1654,6 +1654,8 @@ def sample_codes(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, t
                 return None
             if v.numel() != rows:
                 raise _lib.MqganHipError(f"sample_codes: {name} is a number or has one value per row ({rows}), got {tuple(v.shape)}")
+            if dtype == torch.int32 and v.dtype != dtype:
+                v = v.clamp(-1, V)                  # before 32 bits would wrap it
             held[name] = v.reshape(-1).to(dtype).contiguous()
             return held[name]
         t, k = setting("temperature", temperature, F32), setting("top_k", top_k, torch.int32)
@@ -1706,10 +1708,13 @@ class CodeBalanceFn(torch.autograd.Function):
         ctx.save_for_backward(z, mask, scratch)
         ctx.cfg = (kind, rows, V, stride, logits.shape, sums - at, f - at)
         ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)                             # else zeros are made for the counts
         return loss, counts
 
     @staticmethod
     def backward(ctx, gout, _):
+        if gout is None:
+            return None, None, None, None
         z, mask, scratch = ctx.saved_tensors
         kind, rows, V, stride, shape, sums, f = ctx.cfg
         if torch.is_grad_enabled():

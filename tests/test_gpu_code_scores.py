@@ -152,6 +152,13 @@ def test_draws_among_ties_masks_and_extremes(kind, V):
         check_draws(z, u, **s)
 
 
+def test_draws_with_a_top_k_past_32_bits():
+    from mqgan_amd import ops
+    z, u = torch.randn(4, 100, device=DEV), torch.rand(4, device=DEV)
+    k = torch.tensor([2 ** 32 + 1, -2 ** 40, 2 ** 62, 1], device=DEV)
+    assert torch.equal(ops.sample_codes(z, u, top_k=k), ops.sample_codes(z, u, top_k=torch.tensor([0, 0, 0, 1], dtype=torch.int32, device=DEV)))
+
+
 def test_draws_with_infinite_and_undefined_scores():
     from mqgan_amd import ops
     z = torch.tensor([[0.0, INF, 1.0, INF], [float("nan"), 1.0, float("nan"), -INF], [float("nan")] * 4, [-INF] * 4, [1.0, 2.0, 3.0, 4.0]], device=DEV)
