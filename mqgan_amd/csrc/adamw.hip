@@ -20,6 +20,7 @@ namespace mq {
 
 constexpr int AW_CHUNK = 4096;        // elements a block updates: four groups a wave
 constexpr int AW_NORM = 4;            // chunks a block of the norm reads
+constexpr int64_t AW_MOST = 1 << 24;  // blocks of 256 threads a launch: under 2^32 threads
 constexpr int AW_GRADS = 460;         // gradient addresses a launch carries by value (kernel arguments hold 4 KiB)
 
 struct AwRow {                        // one tensor; the layout of the table is private to this file
@@ -483,7 +484,7 @@ extern "C" size_t mq_adamw_table_bytes(const int64_t *numel_host, int n)
         if (numel_host[i] < 0 || numel_host[i] > (1ll << 50)) return 0;
         blocks += aw_blocks(numel_host[i]);
     }
-    if (blocks >= INT32_MAX) return 0;
+    if (blocks >= AW_MOST) return 0;
     return aw_rows_bytes(n) + (size_t)blocks * sizeof(int);
 }
 
@@ -508,7 +509,7 @@ extern "C" int mq_adamw_table_fill(const mqAdamwTensor *tensors_host, int n, int
                    "mq_adamw_table_fill: tensor %d: parameters start at a multiple of 4 bytes, moments of 16", i);
         MQ_REQUIRE(t.n == 0 || state_bits == 32 || (t.base_avg && t.base_avg_sq), "mq_adamw_table_fill: tensor %d: 8-bit moments need their bases", i);
         blocks += aw_blocks(t.n);
-        MQ_REQUIRE(blocks < INT32_MAX, "mq_adamw_table_fill: too many elements");
+        MQ_REQUIRE(blocks < AW_MOST, "mq_adamw_table_fill: too many elements");
     }
     MQ_REQUIRE(table_bytes == aw_rows_bytes(n) + (size_t)blocks * sizeof(int), "mq_adamw_table_fill: the table has %zu bytes, not %zu",
                aw_rows_bytes(n) + (size_t)blocks * sizeof(int), table_bytes);
@@ -587,7 +588,7 @@ extern "C" int mq_moments8_encode(const float *exp_avg, const float *exp_avg_sq,
 {
     MQ_REQUIRE(exp_avg && exp_avg_sq && codes_avg && base_avg && codes_avg_sq && base_avg_sq && n > 0 && n % 256 == 0, "mq_moments8_encode: bad arguments (n is a multiple of 256)");
     MQ_REQUIRE(((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq) % 16 == 0 && ((uintptr_t)codes_avg | (uintptr_t)codes_avg_sq) % 4 == 0, "mq_moments8_encode: moments start at multiples of 16 bytes, codes of 4");
-    MQ_REQUIRE(cdiv(n, 1024) < INT32_MAX, "mq_moments8_encode: too many elements");
+    MQ_REQUIRE(cdiv(n, 1024) < AW_MOST, "mq_moments8_encode: too many elements");
     hipLaunchKernelGGL(moments8_encode_kernel, dim3((unsigned)cdiv(n, 1024)), dim3(256), 0, S(stream), exp_avg, exp_avg_sq, n / 256,
                        reinterpret_cast<uint32_t *>(codes_avg), base_avg, reinterpret_cast<uint32_t *>(codes_avg_sq), base_avg_sq);
     MQ_LAUNCH_CHECK("mq_moments8_encode");
@@ -600,7 +601,7 @@ extern "C" int mq_moments8_decode(const uint8_t *codes_avg, const uint8_t *base_
     MQ_REQUIRE(codes_avg && base_avg && codes_avg_sq && base_avg_sq && exp_avg && exp_avg_sq && n > 0 && n % 256 == 0, "mq_moments8_decode: bad arguments (n is a multiple of 256)");
     MQ_REQUIRE(((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq) % 16 == 0 && ((uintptr_t)codes_avg | (uintptr_t)codes_avg_sq) % 8 == 0, "mq_moments8_decode: moments start at multiples of 16 bytes, codes of 8");
     const int64_t n8 = n / 8;
-    MQ_REQUIRE(cdiv(n8, 256) < INT32_MAX, "mq_moments8_decode: too many elements");
+    MQ_REQUIRE(cdiv(n8, 256) < AW_MOST, "mq_moments8_decode: too many elements");
     const uint2 *mc = reinterpret_cast<const uint2 *>(codes_avg), *vc = reinterpret_cast<const uint2 *>(codes_avg_sq);
     if (bf16)
         hipLaunchKernelGGL(moments8_decode_kernel<true>, dim3((unsigned)cdiv(n8, 256)), dim3(256), 0, S(stream), mc, base_avg, vc, base_avg_sq, n8, exp_avg, exp_avg_sq);

@@ -38,7 +38,7 @@ struct SampleArgs {
     const uint8_t *padded;
     int64_t *idx;
     float *logp;
-    int64_t rows;
+    int64_t row0, rows;                                              // those of a launch: [row0, rows)
     int squeezes;                                                    // the rows' LDS has room for V indices
     __device__ __forceinline__ double T(int64_t n) const { return temperature ? (double)temperature[n] : t0; }
     __device__ __forceinline__ double P(int64_t n) const { return top_p ? (double)top_p[n] : p0; }
@@ -815,7 +815,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 6 : W == 1 ? 5 : 4) void sample_ke
     __shared__ Shared<W, W == 1 ? 128 : 256> s;
     __shared__ Few<DT, KEPT> few;
     Raw *lds = reinterpret_cast<Raw *>(staged);
-    draw_row<DT, HELD, W>(a, blockIdx.x, lds, s, a.squeezes ? reinterpret_cast<uint16_t *>(lds + (a.V + 3) / 4 * 4) : nullptr, &few);
+    draw_row<DT, HELD, W>(a, a.row0 + blockIdx.x, lds, s, a.squeezes ? reinterpret_cast<uint16_t *>(lds + (a.V + 3) / 4 * 4) : nullptr, &few);
 }
 
 // For many rows with top-k: a block takes W of them, one after the other as far as it needs the whole row - the next one is on its way
@@ -831,7 +831,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 6 : 4) void sample_many_kernel(con
     __shared__ Shared<W, 256> s;
     __shared__ F few[W];
     const int V = a.V, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    const int64_t n0 = (int64_t)blockIdx.x * W;
+    const int64_t n0 = a.row0 + (int64_t)blockIdx.x * W;
     const int rows = (int)min((int64_t)W, a.rows - n0);
     typename S::Raw *lds = reinterpret_cast<typename S::Raw *>(staged);
     const auto answer = [&](int r, int64_t i, float lp) {
@@ -935,20 +935,20 @@ static void sample_go(SampleArgs a, hipStream_t s)
 {
     const size_t row = row_bytes<DT>(a.V), index = (size_t)a.V * sizeof(uint16_t);
     a.squeezes = row + index <= ROOM && (a.top_k || a.k0 > 0 || a.top_p || a.p0 < 1.0);
-    hipLaunchKernelGGL((sample_kernel<DT, true, W>), dim3((unsigned)a.rows), dim3(64 * W), row + (a.squeezes ? index : 0), s, a);
+    hipLaunchKernelGGL((sample_kernel<DT, true, W>), dim3((unsigned)(a.rows - a.row0)), dim3(64 * W), row + (a.squeezes ? index : 0), s, a);
 }
 template <int DT, int W>
 static void sample_many(const SampleArgs &a, hipStream_t s)
 {
-    hipLaunchKernelGGL((sample_many_kernel<DT, W>), dim3((unsigned)((a.rows + W - 1) / W)), dim3(64 * W), std::max(row_bytes<DT>(a.V), W * sizeof(Search<128>)), s, a);
+    hipLaunchKernelGGL((sample_many_kernel<DT, W>), dim3((unsigned)((a.rows - a.row0 + W - 1) / W)), dim3(64 * W), std::max(row_bytes<DT>(a.V), W * sizeof(Search<128>)), s, a);
 }
 template <int DT>
 static void sample_launch(const SampleArgs &a, hipStream_t s)
 {
     const bool list = a.top_k || (a.k0 > 0 && a.k0 <= 128) || (!a.temperature && a.t0 == 0.0);
-    if (a.V > 16384 || row_bytes<DT>(a.V) > ROOM) hipLaunchKernelGGL((sample_kernel<DT, false, 8>), dim3((unsigned)a.rows), dim3(512), 0, s, a);
-    else if (a.rows < 256 && a.V <= 1024) sample_go<DT, 4>(a, s);
-    else if (a.rows < 256 || a.V > 8192) sample_go<DT, 16>(a, s);
+    if (a.V > 16384 || row_bytes<DT>(a.V) > ROOM) hipLaunchKernelGGL((sample_kernel<DT, false, 8>), dim3((unsigned)(a.rows - a.row0)), dim3(512), 0, s, a);
+    else if (a.rows - a.row0 < 256 && a.V <= 1024) sample_go<DT, 4>(a, s);
+    else if (a.rows - a.row0 < 256 || a.V > 8192) sample_go<DT, 16>(a, s);
     else if (a.V <= 1024) sample_go<DT, 1>(a, s);
     else if (a.V <= 4096) list ? sample_many<DT, 4>(a, s) : sample_go<DT, 4>(a, s);
     else list ? sample_many<DT, 8>(a, s) : sample_go<DT, 8>(a, s);
@@ -968,10 +968,14 @@ extern "C" int mq_sample_codes(const mqSampleDesc *d, const void *logits, const 
     int bits = 0;
     while ((1ll << bits) < d->codes) ++bits;
     const int shift = 62 - bits < 51 ? 62 - bits : 51;
-    const SampleArgs a{logits, d->row_stride, d->codes, shift, uniform, temperature, top_p, min_p, top_k, d->temperature, d->top_p, d->min_p, d->top_k, padded, idx, logp, d->rows, 0};
-    if (d->dtype == 0) sample_launch<0>(a, S(stream));
-    else if (d->dtype == 1) sample_launch<1>(a, S(stream));
-    else sample_launch<2>(a, S(stream));
+    SampleArgs a{logits, d->row_stride, d->codes, shift, uniform, temperature, top_p, min_p, top_k, d->temperature, d->top_p, d->min_p, d->top_k, padded, idx, logp, 0, 0, 0};
+    constexpr int64_t MOST = 1 << 21;                               // rows a launch: one holds under 2^32 threads
+    for (a.row0 = 0; a.row0 < d->rows; a.row0 = a.rows) {
+        a.rows = std::min(a.row0 + MOST, d->rows);
+        if (d->dtype == 0) sample_launch<0>(a, S(stream));
+        else if (d->dtype == 1) sample_launch<1>(a, S(stream));
+        else sample_launch<2>(a, S(stream));
+    }
     MQ_LAUNCH_CHECK("mq_sample_codes");
     return 0;
 }

@@ -87,6 +87,10 @@ class AdamW:
         if torch.cuda.is_current_stream_capturing():
             raise MqganHipError("AdamW: a parameter moved since the last step; take one step outside the capture first")
         n, item = len(self.params), self.exp_avg.element_size()
+        spans = sorted((a, a + 4 * s, i) for i, (a, s) in enumerate(zip(addresses, self._sizes)) if s)
+        for (_, end, i), (start, _, j) in zip(spans, spans[1:]):
+            if start < end:
+                raise MqganHipError(f"AdamW: parameters {i} and {j} share memory")
         m, v = self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr()
         mb, vb = (b.data_ptr() for b in self._bases) if self._bases else (0, 0)
         rows = (AdamwTensor * n)()

@@ -378,9 +378,11 @@ def test_refusals():
             bad()
     opt = AdamW([p])
     for bad in (lambda: AdamW([torch.zeros(8)]), lambda: AdamW([p.half()]), lambda: AdamW([torch.zeros(8, 8, device=DEV).t()]),
+                lambda: AdamW([p[:5], p[4:]]), lambda: AdamW([p, p.detach()]),
                 lambda: opt.step(grads=[]), lambda: opt.step(grads=[torch.zeros(7, device=DEV)]), lambda: opt.step(grads=[torch.zeros(8)]),
                 lambda: opt.step(grads=[torch.zeros(8, device=DEV, dtype=torch.float64)]), lambda: opt.load_moments(p, p),
                 lambda: AdamW([p], state_bits=8).moments(torch.float16)):
         with pytest.raises(MqganHipError):
             bad()
     assert opt._steps() == ([0], 0)
+    AdamW([p[:4], p[4:], torch.zeros(0, device=DEV)])      # halves of one buffer are two parameters

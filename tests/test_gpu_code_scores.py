@@ -100,6 +100,7 @@ def test_draws_of_many_rows_equal_those_of_few(V):
         z[5::7] *= 0.01                                              # flat: top-p keeps most
         z[torch.rand(n, V, generator=g) < 0.1] = -INF
         z[3], z[40, V // 2], z[41] = -INF, INF, 2.5
+        z[42, ::2], z[43], z[44] = torch.finfo(torch.float32).min, z[43] * 1e4, z[44].clamp(0, 0) * z[44].sign()      # zeros of both signs
         z, u = z.to(dtype).to(DEV), torch.rand(n, generator=g).to(DEV)
         padded = (torch.rand(n, generator=g) < 0.1).to(DEV)
         by_row = {"temperature": torch.rand(n, generator=g).to(DEV) * 2 - 0.2, "top_p": torch.rand(n, generator=g).to(DEV),
@@ -150,6 +151,20 @@ def test_draws_among_ties_masks_and_extremes(kind, V):
     u[0], u[1] = 0.0, 1 - 2.0 ** -24
     for s in SETTINGS:
         check_draws(z, u, **s)
+
+
+def test_draws_of_more_rows_than_one_launch_takes():
+    from mqgan_amd import ops
+    g = torch.Generator(device=DEV).manual_seed(8)
+    n = (1 << 21) + 5
+    z, u = torch.randn(n, 3, device=DEV, generator=g), torch.rand(n, device=DEV, generator=g)
+    idx, logp = ops.sample_codes(z, u, top_k=2, return_logp=True)
+    half = 1 << 20
+    for at in range(0, n, half):
+        i, lp = ops.sample_codes(z[at:at + half], u[at:at + half], top_k=2, return_logp=True)
+        assert torch.equal(i, idx[at:at + half]) and torch.equal(lp, logp[at:at + half])
+    last = z.sort(dim=-1, descending=True, stable=True).indices[:, -1]      # of two equal lowest the one with the higher index
+    assert int(idx.min()) >= 0 and not bool((idx == last).any())
 
 
 def test_draws_with_a_top_k_past_32_bits():

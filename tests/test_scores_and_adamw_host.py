@@ -75,6 +75,7 @@ def test_adamw_refuses_on_the_host(lib):
     assert nbytes == 192 + 3 * 4 and lib.mq_adamw_control_bytes(2) == 96 and lib.mq_adamw_workspace(sizes, 2) >= 3 * 8
     assert lib.mq_adamw_table_bytes((C.c_int64 * 1)(-1), 1) == 0 and lib.mq_adamw_table_bytes(sizes, 0) == 0
     assert lib.mq_adamw_table_bytes((C.c_int64 * 1)(2 ** 63 - 1), 1) == 0
+    assert lib.mq_adamw_table_bytes((C.c_int64 * 1)(2 ** 36 - 4096), 1) > 0 and lib.mq_adamw_table_bytes((C.c_int64 * 1)(2 ** 36 - 4095), 1) == 0      # 2^32 threads
 
     def fill(bits=32, count=2, size=nbytes, host=True, **kw):
         rows = (AdamwTensor * 2)(AdamwTensor(4096, 8192, 16384, 100, 200, 300, 0, 0.0, 1.0), AdamwTensor(4096, 8192, 16384, 100, 200, 5000, 512, 0.1, 1.0))
@@ -116,6 +117,8 @@ def test_adamw_refuses_on_the_host(lib):
     refused(lib, lib.mq_moments8_encode(A, None, 256, A, A, A, A, None), b"bad arguments")
     refused(lib, lib.mq_moments8_encode(C.c_void_p(4100), A, 256, A, A, A, A, None), b"multiples")
     refused(lib, lib.mq_moments8_decode(A, A, A, A, 100, 0, A, A, None), b"256")
+    refused(lib, lib.mq_moments8_encode(A, A, 2 ** 34, A, A, A, A, None), b"too many")
+    refused(lib, lib.mq_moments8_decode(A, A, A, A, 2 ** 35, 0, A, A, None), b"too many")
     refused(lib, lib.mq_moments8_decode(A, A, A, A, 256, 0, A, C.c_void_p(4104), None), b"multiples")
 
 
