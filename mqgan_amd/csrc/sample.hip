@@ -140,20 +140,22 @@ struct Row {
     double max, per_t;                   // 1 / T; 0 for T = inf
     double per2;                         // log2(e) / T
     int shift;                           // weights are w 2^shift
-    double least;                        // min_p 2^shift, min_p <= 1
+    double tiny, least;                  // 2^shift times the smallest weight above 0, and times min_p where that is more (min_p <= 1)
     __device__ __forceinline__ Row(float max_, double T, double min_p, int shift_)
-        : max((double)max_), per_t(fmin(1.0 / T, 1e300)), per2(per_t * 1.4426950408889634074), shift(shift_), least(ldexp(min_p > 1.0 ? 1.0 : min_p, shift_))
+        : max((double)max_), per_t(fmin(1.0 / T, 1e300)), per2(per_t * 1.4426950408889634074), shift(shift_), tiny(ldexp(1.15, shift_ - 1075)),
+          least(fmax(ldexp(min_p > 1.0 ? 1.0 : min_p, shift_), tiny))
     {
     }
     // Units of a code with a score above -inf: w 2^shift to the nearest whole number, at least 1 - the bits of w 2^shift + 2^52 (shift <= 51,
-    // w <= 1); 0 where w would underflow in f64 and where w 2^shift is under `limit`.
-    __device__ __forceinline__ uint64_t units(float x, double limit = 0.0) const
+    // w <= 1); 0 where w would underflow in f64 (also where d is past f64, w a NaN) and where w 2^shift is under `limit`.
+    __device__ __forceinline__ uint64_t units(float x, double limit) const
     {
-        const double d = ((double)x - max) * per2, c = fmax(d, -1100.0), n = rint(c);
-        const double w = ldexp(exp2_half(c - n), (int)n + shift);
+        const double d = ((double)x - max) * per2, n = rint(d);
+        const double w = ldexp(exp2_half(d - n), (int)n + shift);
         const uint64_t q = (uint64_t)__double_as_longlong(fmax(w, 1.0) + 4503599627370496.0) & 0xfffffffffffffull;
-        return d < -1074.8 || w < limit ? 0 : q;
+        return w >= limit ? q : 0;
     }
+    __device__ __forceinline__ uint64_t units(float x) const { return units(x, tiny); }
     // log of a weight's share of Z units
     __device__ __forceinline__ float logp(float x, uint64_t Z) const { return (float)(((double)x - max) * per_t - ln(ldexp((double)Z, -shift))); }
 };
@@ -272,6 +274,7 @@ struct Search {
     Entry list[LIST];                                               // codes of the bin that a cut falls into
     float cut_x;
     int cut_i, length;
+    unsigned long long cut_mass;                                    // up to and with the cut
     Found found;
 };
 // The codes kept of a row, in index order, once they are few, and the row's settings
@@ -392,6 +395,7 @@ struct Draw {
         const float border = score_of((uint32_t)prefix);
         const uint64_t w = q(border);
         const int need = (int)((goal - above + w - 1) / w);
+        if (threadIdx.x % NT == 0) s.cut_mass = above + (uint64_t)need * w;
         const int lane = threadIdx.x & 63, c0 = begin, c1 = end;
         uint32_t mine = 0;
         each([&](float v, int) { mine += v == border; });
@@ -476,6 +480,7 @@ struct Draw {
             if (before < goal && before + me.w >= goal) {
                 s.cut_x = me.x;
                 s.cut_i = me.i;
+                s.cut_mass = before + me.w;
             }
         }
         together<W>();
@@ -488,6 +493,7 @@ struct Draw {
     __device__ __forceinline__ void finish(const Row &r, float mx, int k, double P, float u, uint64_t Z, A answer)
     {
         const int lane = threadIdx.x & 63;
+        bool known = false;                                         // whether cut_mass is the kept mass
 #pragma unroll 1
         for (int stage = 0; stage < 2; ++stage) {                   // one copy of find_cut for both: the code has to stay in the instruction cache
             uint64_t goal = (uint64_t)k;
@@ -498,12 +504,14 @@ struct Draw {
                 if (!Z) Z = total(sum([&](float v) { return r.units(v); }));
                 goal = goal_of(P, Z);
             }
-            find_cut(mx, goal, [&](float v) { return stage == 0 ? (uint64_t)1 : r.units(v); });
+            const bool found = find_cut(mx, goal, [&](float v) { return stage == 0 ? (uint64_t)1 : r.units(v); });
+            known = stage == 1 && found;
         }
-        // the waves' sums, then the wave that the draw falls to goes over its part again (NaN min_p: nothing is under it)
-        const uint64_t part_ = wave_total(sum([&](float v) { return r.units(v, r.least); }));
+        // the waves' sums, then the wave that the draw falls to goes over its part again (NaN min_p: nothing is under it); a wave by itself has
+        // the sum from the cut already
+        const uint64_t own = W == 1 && known && r.least == r.tiny ? s.cut_mass : wave_total(sum([&](float v) { return r.units(v, r.least); }));
         together<W>();
-        if (lane == 0) red[wave()] = part_;
+        if (lane == 0) red[wave()] = own;
         together<W>();
         uint64_t mass = 0;
 #pragma unroll
