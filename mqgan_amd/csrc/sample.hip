@@ -12,14 +12,21 @@
 // same way on every run.  With f32 masses a row of 8192 codes would be drawn next to a border about once in 1000 rows.  A weight under
 // the unit counts as one unit (2^-49 at V = 8192) unless exp gives 0.
 //
-// Both cuts are a place in the order, (score, index): everything at or before it stays.  A block has one row; where it fits (48 KiB) the row is
-// read once, into LDS.  Mostly a bound tells that the first cut lies among few codes - k of the threads' own maxima are at least so large; the
-// codes beyond some distance hold less mass than top_p leaves out - and then these become a list, in index order, that one wave works
-// on alone: the blocks' barriers were what the time went into.  A cut is found without sorting: a histogram over the distance from the maximum
-// (bins of equal RATIO, so neither the scores' scale nor masks of the type's lowest value matter) tells the bin that it falls into, a second
-// one over that bin's lower bits narrows it, and the few codes left are put into a list and counted against each other.  Where that list
-// overflows (hundreds of equal scores across the cut) radix selection over the bits of the score finds the cut instead.
-// A wave covers a contiguous part of the row, so that sums up to a code need one number per wave.
+// Both cuts are a place in the order, (score, index): everything at or before it stays.  A block has one row, which is read once, into LDS, where
+// it fits (up to 14336 f32 or 16384 two-byte scores); each wave has a contiguous part, reads back what it wrote itself and needs no barrier
+// for that, and sums up to a code need one number per wave.  The codes that can be before a cut are found by a bound first - k of the threads'
+// own maxima are at least so large; codes beyond some distance hold less mass than top_p leaves out - and packed, in index order.
+// A cut is found without sorting: a histogram over the distance from the maximum (bins of equal RATIO, so neither the scores' scale nor masks of
+// the type's lowest value matter) tells the bin that it falls into, a second one over that bin's lower bits narrows it, and the few codes left
+// are put into a list and counted against each other.  Where that list overflows (dozens of equal scores across the cut) radix selection over
+// the bits of the score finds the cut instead.
+//
+// What bounds it: 16384 x 8192 f32 read once are 76 us at the 7.1 TB/s that loads alone reach here.  The maximum alone (temperature 0) takes 105 us,
+// top-k 20 147, top-k 100 with top-p 0.95 210: 70 % of the latter is the issue of vector instructions (6000 per row and wave slot), the rest
+// waits of the lists' waves.  Without top-k the masses of all codes are needed, 22 f64 operations each, twice for the one that is drawn: 16384 x
+// 8192 without a filter 280 us, top-p 0.95 530; 16384 x 1024 with top-p 0.9 65 (floor 9.5), 85 % of it vector issue.  Small calls are latency:
+// one row of 1000 codes with all filters 9 us, 48 of 8003 with top-p 0.95 26 us, a chain of some thirty dependent LDS accesses and barriers.
+// A register-resident row (215 registers, one block a compute unit) took 2.6 times as long, sorting-free selection by bits alone 11 times.
 #include <algorithm>
 
 #include "common.h"
@@ -828,7 +835,8 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 6 : W == 1 ? 5 : 4) void sample_ke
 
 // For many rows with top-k: a block takes W of them, one after the other as far as it needs the whole row - the next one is on its way
 // meanwhile - and what is done on a short list of codes is left to the end, where each wave has a row's.  Rows without such a list
-// come last, by the whole block.
+// come last, by the whole block.  One row a block and its list by one wave took 334 us where this takes 210 (16384 x 8192, top-k 100 and
+// top-p 0.95): the row's 32 KB of LDS were held while seven of eight waves had nothing to do.
 template <int DT, int W>
 __global__ __launch_bounds__(64 * W, W == 8 ? 6 : 4) void sample_many_kernel(const SampleArgs a)
 {
@@ -950,16 +958,25 @@ static void sample_many(const SampleArgs &a, hipStream_t s)
 {
     hipLaunchKernelGGL((sample_many_kernel<DT, W>), dim3((unsigned)((a.rows - a.row0 + W - 1) / W)), dim3(64 * W), std::max(row_bytes<DT>(a.V), W * sizeof(Search<128>)), s, a);
 }
+// Waves a row: fewer with more rows, whose waves fill the chip without barriers between them.  Measured (f32, normal scores with deviation 3;
+// us without a filter / top-p 0.95 / top-k 100 and top-p 0.95):
+//   1000 codes: 1024 rows 7.0 / 16.0 / 17.5 with four waves, 8.0 / 19.0 / 19.3 with one; 4096 rows 17.6 / 41.6 / 31.9, 14.8 / 29.2 / 27.7
+//   4096 codes: 256 rows 6.8 / 13.8 / 17.0 with eight, 8.3 / 17.5 / 17.8 with four; 1024 rows 13.5 / 29.1 / 24.0, 13.7 / 26.9 / 20.1
+//   8192 codes: 256 rows 8.7 / 18.5 / 20.1 with sixteen, 9.4 / 19.9 / 17.8 with eight; 512 rows 14.1 / 33.6 / 36.0, 12.4 / 26.0 / 19.7
+// The kernel for many rows wants enough of them for every compute unit (top-k 100 and top-p 0.95: 8192 codes, 2048 rows 71 against 55 us, 4096 87
+// against 100; 4096 codes, 2048 rows 33 against 36, 4096 43 against 66; 2048 codes never pays) and a k whose list is short (8192 codes, 16384
+// rows: k = 128 199 us, k = 160 436 against 263; 4096 codes, 4096 rows: k = 100 43 against 66, k = 128 47 against 45).
 template <int DT>
 static void sample_launch(const SampleArgs &a, hipStream_t s)
 {
-    const bool list = a.top_k || (a.k0 > 0 && a.k0 <= 128) || (!a.temperature && a.t0 == 0.0);
-    if (a.V > 16384 || row_bytes<DT>(a.V) > ROOM) hipLaunchKernelGGL((sample_kernel<DT, false, 8>), dim3((unsigned)(a.rows - a.row0)), dim3(512), 0, s, a);
-    else if (a.rows - a.row0 < 256 && a.V <= 1024) sample_go<DT, 4>(a, s);
-    else if (a.rows - a.row0 < 256 || a.V > 8192) sample_go<DT, 16>(a, s);
-    else if (a.V <= 1024) sample_go<DT, 1>(a, s);
-    else if (a.V <= 4096) list ? sample_many<DT, 4>(a, s) : sample_go<DT, 4>(a, s);
-    else list ? sample_many<DT, 8>(a, s) : sample_go<DT, 8>(a, s);
+    const int64_t n = a.rows - a.row0;
+    const int k = a.top_k ? 0 : a.k0;
+    const bool greedy = !a.temperature && a.t0 == 0.0;
+    if (a.V > 16384 || row_bytes<DT>(a.V) > ROOM) hipLaunchKernelGGL((sample_kernel<DT, false, 8>), dim3((unsigned)n), dim3(512), 0, s, a);
+    else if (a.V <= 1024) n < 2048 ? sample_go<DT, 4>(a, s) : sample_go<DT, 1>(a, s);
+    else if (a.V <= 4096) n <= 512 ? sample_go<DT, 8>(a, s) : n >= 4096 && a.V > 2048 && k > 0 && k <= 100 ? sample_many<DT, 4>(a, s) : sample_go<DT, 4>(a, s);
+    else if (a.V <= 8192) n <= 256 && k <= 0 ? sample_go<DT, 16>(a, s) : n >= 4096 && (greedy || (k > 0 && k <= 128)) ? sample_many<DT, 8>(a, s) : sample_go<DT, 8>(a, s);
+    else sample_go<DT, 16>(a, s);
 }
 
 extern "C" int mq_sample_codes(const mqSampleDesc *d, const void *logits, const float *uniform, const float *temperature, const int32_t *top_k,

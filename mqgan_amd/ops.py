@@ -1664,7 +1664,7 @@ def sample_codes(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, t
         d = _lib.SampleDesc(rows, stride, V, kind, 0.0 if t is not None else float(temperature), 0.0 if p is not None else float(top_p),
                             0.0 if m is not None else float(min_p), 0 if k is not None else min(int(top_k), V))
         check(L().mq_sample_codes(C.byref(d), _score_ptr(z), fptr(u), fptr(t, True), ptr(k, torch.int32, True), fptr(p, True), fptr(m, True),
-                                  ptr(mask, None, True), ptr(idx, torch.int64), fptr(logp, True), stream()), "mq_sample_codes")
+                                  ptr(mask, None, True), idx.data_ptr(), None if logp is None else logp.data_ptr(), stream()), "mq_sample_codes")
     return (idx, logp) if return_logp else idx
 
 
@@ -1688,13 +1688,13 @@ class CodeBalanceFn(torch.autograd.Function):
         scratch = _empty((n_stats + n_sums + V + 3 + nbytes // 4,), z)
         counts = torch.empty((V,), dtype=torch.int32, device=z.device)
         loss = _empty((), z)
-        zp, at = _score_ptr(z), fptr(scratch).value
+        zp, at, lp = _score_ptr(z), scratch.data_ptr(), loss.data_ptr()
         sums, f, ws = at + 4 * n_stats, at + 4 * (n_stats + n_sums), at + 4 * (n_stats + n_sums + (V + 3) // 4 * 4)
         together = comm is not None and comm.active
         if rows:
             idx = idx.contiguous()
             check(lib.mq_code_balance_fwd(zp, kind, stride, ptr(idx), int(idx.dtype == torch.int64), K, ptr(mask, None, True), rows, V, at,
-                                          ptr(counts), sums, None if together else fptr(loss), None if together else f, ws, nbytes, stream()),
+                                          counts.data_ptr(), sums, None if together else lp, None if together else f, ws, nbytes, stream()),
                   "mq_code_balance_fwd")
         else:
             scratch.zero_()
@@ -1704,7 +1704,7 @@ class CodeBalanceFn(torch.autograd.Function):
                 s = scratch[n_stats:n_stats + 2 * V + 1]
                 _reduce(comm, s)
                 counts = s[V:2 * V].to(torch.int32)
-            check(lib.mq_code_balance_final(sums, V, K, fptr(loss), f, stream()), "mq_code_balance_final")
+            check(lib.mq_code_balance_final(sums, V, K, lp, f, stream()), "mq_code_balance_final")
         ctx.save_for_backward(z, mask, scratch)
         ctx.cfg = (kind, rows, V, stride, logits.shape, sums - at, f - at)
         ctx.mark_non_differentiable(counts)
@@ -1722,7 +1722,7 @@ class CodeBalanceFn(torch.autograd.Function):
         dz = torch.empty(shape, dtype=z.dtype, device=z.device)
         if rows:
             at = scratch.data_ptr()
-            check(L().mq_code_balance_bwd(_score_ptr(z), kind, stride, ptr(mask, None, True), rows, V, at, at + sums, at + f, fptr(gout), ptr(dz),
+            check(L().mq_code_balance_bwd(_score_ptr(z), kind, stride, ptr(mask, None, True), rows, V, at, at + sums, at + f, fptr(gout), dz.data_ptr(),
                                           stream()), "mq_code_balance_bwd")
         return dz, None, None, None
 

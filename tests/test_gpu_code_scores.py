@@ -88,37 +88,36 @@ def test_draws_follow_the_definition(V, dtype):
         check_draws(z, u, **s)
 
 
-@pytest.mark.parametrize("V", [1, 3, 255, 256, 260, 1000, 1024, 1025, 2047, 4096, 4097, 8003, 8192, 8193, 9000, 16384, 16385])
-def test_draws_of_many_rows_equal_those_of_few(V):
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("V", [1, 3, 255, 256, 260, 1000, 1024, 1025, 2047, 4096, 4097, 8003, 8192, 8193, 9000, 14336, 14337, 16384, 16385])
+def test_draws_of_many_rows_equal_those_of_few(V, dtype):
     """Masses are whole numbers, so however a row's work is split its code and its logarithm are the same to the last bit; and the definition's."""
     from mqgan_amd import ops
-    g = torch.Generator().manual_seed(V + 5)
-    n, few = 301, 50
-    for dtype in (torch.float32, torch.bfloat16):
-        z = torch.randn(n, V, generator=g) * 3
-        z[::7] = (z[::7] * 2).round()                                # ties
-        z[5::7] *= 0.01                                              # flat: top-p keeps most
-        z[torch.rand(n, V, generator=g) < 0.1] = -INF
-        z[3], z[40, V // 2], z[41] = -INF, INF, 2.5
-        z[42, ::2], z[43], z[44] = torch.finfo(torch.float32).min, z[43] * 1e4, z[44].clamp(0, 0) * z[44].sign()      # zeros of both signs
-        z, u = z.to(dtype).to(DEV), torch.rand(n, generator=g).to(DEV)
-        padded = (torch.rand(n, generator=g) < 0.1).to(DEV)
-        by_row = {"temperature": torch.rand(n, generator=g).to(DEV) * 2 - 0.2, "top_p": torch.rand(n, generator=g).to(DEV),
-                  "top_k": torch.randint(-1, 200, (n,), generator=g, dtype=torch.int32).to(DEV)}
-        for s in SETTINGS + [{"top_k": 90, "top_p": 0.95}, {"top_k": 200}, by_row, {"temperature": by_row["temperature"], "top_k": 30}]:
-            s = dict(s, padded=padded)
-            idx, logp = ops.sample_codes(z, u, return_logp=True, **s)
-            for at in range(0, n, few):
-                part = {k: v[at:at + few] if torch.is_tensor(v) else v for k, v in s.items()}
-                i, lp = ops.sample_codes(z[at:at + few], u[at:at + few], return_logp=True, **part)
-                assert torch.equal(i, idx[at:at + few]) and torch.equal(lp, logp[at:at + few]), (s, at)
-        rows = torch.arange(0, n, 20, device=DEV)
-        big = torch.randn(n, V, generator=g).to(dtype).to(DEV)
-        for s in ({}, {"top_k": 20, "top_p": 0.9}, {"top_p": 0.7, "min_p": 0.01}):
-            idx = ops.sample_codes(big, u, **s)
-            for r in rows.tolist():
-                want, _, margin = ref_row(big[r].float().cpu().numpy(), float(u[r]), **{{"top_k": "k", "top_p": "p", "min_p": "mp"}[k]: v for k, v in s.items()})
-                assert 0 < margin < 1e-9 or int(idx[r]) == want, (s, r)
+    g = torch.Generator(device=DEV).manual_seed(V + 5)
+    n = 4101
+    rand = lambda *s: torch.rand(*s, generator=g, device=DEV)  # noqa: E731
+    normal = torch.randn(n, V, generator=g, device=DEV) * 3
+    z = normal.clone()
+    z[::7] = (z[::7] * 2).round()                                # ties
+    z[5::7] *= 0.01                                              # flat: top-p keeps most
+    z[rand(n, V) < 0.1] = -INF
+    z[3], z[40, V // 2], z[41] = -INF, INF, 2.5
+    z[42, ::2], z[43], z[44] = torch.finfo(torch.float32).min, z[43] * 1e4, z[44].clamp(0, 0) * z[44].sign()      # zeros of both signs
+    z, normal, u, padded = z.to(dtype), normal.to(dtype), rand(n), rand(n) < 0.1
+    padded[40:45] = False
+    by_row = {"temperature": rand(n) * 2 - 0.2, "top_p": rand(n), "top_k": torch.randint(-1, 200, (n,), generator=g, device=DEV, dtype=torch.int32)}
+    for s in SETTINGS + [{"top_k": 90, "top_p": 0.95}, {"top_k": 120}, {"top_k": 200}, by_row, {"temperature": by_row["temperature"], "top_k": 30}]:
+        s = dict(s, padded=padded)
+        idx, logp = ops.sample_codes(z, u, return_logp=True, **s)
+        for a, b in ((0, 50), (50, 350), (350, 1000), (1000, 3100), (3100, n)):
+            part = {k: v[a:b] if torch.is_tensor(v) else v for k, v in s.items()}
+            i, lp = ops.sample_codes(z[a:b], u[a:b], return_logp=True, **part)
+            assert torch.equal(i, idx[a:b]) and torch.equal(lp, logp[a:b]), (s, a)
+    for s in ({}, {"top_k": 20, "top_p": 0.9}, {"top_p": 0.7, "min_p": 0.01}):
+        idx = ops.sample_codes(normal, u, **s)
+        for r in range(0, n, 400):
+            want, _, margin = ref_row(normal[r].float().cpu().numpy(), float(u[r]), **{{"top_k": "k", "top_p": "p", "min_p": "mp"}[k]: v for k, v in s.items()})
+            assert 0 < margin < 1e-9 or int(idx[r]) == want, (s, r)
 
 
 @pytest.mark.parametrize("kind", ["levels", "equal", "zeros of both signs", "masked", "one left", "lowest of the type", "steep", "falling", "rising"])
