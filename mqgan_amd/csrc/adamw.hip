@@ -14,6 +14,12 @@
 // the rest is cut off.  To nearest, a second moment with b2 = 0.999 would not move at all - its change per step, 0.1 % of
 // (g'^2 - v), is far under half a step of a 3-bit mantissa (3-6 %); rounded at random it moves by the right amount on average.  The
 // bits are a hash of (seed, call, position in the moments' layout): the same on every replay of a run.
+//
+// All of it is bound by memory.  f32 moments: 28 bytes an element with f32 gradients, plus 4 for the norm, whose pass
+// leaves part of the gradients in the 256 MB cache.  34 M elements in 260 tensors: update 142 us (6.7 TB/s), norm 27, factors 5, where
+// the same passes as tensor operations take 1510.  8 bits: 16.02 bytes, 87 us (6.3 TB/s) + norm 33; 150 M elements with bf16 gradients 353-371 us
+// (14.02 bytes, 5.8 TB/s) + norm 70-94.  Chunks of 4096 elements as straight-line code with all loads issued first took the f32 update from 170 to 142;
+// codes by shifts in place of compares and the hardware's root and reciprocal took an 8-bit step of 34 M with its moments decoded from 202 to 168.
 #include "common.h"
 
 namespace mq {

@@ -27,7 +27,8 @@ thread_local char g_kernel[128] = "";
 //    test-variant build alone (make variants), which also carries the rejected kernel variants; the two hooks are named
 //    mq_debug_set_*_hook; the screened codebook search's bound comes from measured rounding residuals
 // 11: mq_comm_unique_id / mq_comm_init / mq_allreduce_bucket / mq_comm_destroy (the gradient-bucket all-reduce over RCCL, resolved
-//    with dlopen at first use: csrc/collective.cpp)
+//    with dlopen at first use: csrc/collective.cpp); later additions only, nothing that was there changed: mq_code_balance_*,
+//    mq_sample_codes, mq_adamw_* and mq_moments8_*
 extern "C" int mq_abi_version(void) { return 11; }
 extern "C" const char *mq_last_error(void) { return mq::g_err; }
 extern "C" const char *mq_last_kernel(void) { return mq::g_kernel; }
