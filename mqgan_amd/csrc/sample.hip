@@ -153,8 +153,8 @@ struct Row {
           least(fmax(ldexp(min_p > 1.0 ? 1.0 : min_p, shift_), tiny))
     {
     }
-    // Units of a code with a score above -inf: w 2^shift to the nearest whole number, at least 1 - the bits of w 2^shift + 2^52 (shift <= 51,
-    // w <= 1); 0 where w would underflow in f64 (also where d is past f64, w a NaN) and where w 2^shift is under `limit`.
+    // Units of a code: w 2^shift to the nearest whole number, at least 1 - the bits of w 2^shift + 2^52 (shift <= 51, w <= 1); 0 where w would
+    // underflow in f64 (where d is past f64, as for a score of -inf, w is a NaN) and where w 2^shift is under `limit`.
     __device__ __forceinline__ uint64_t units(float x, double limit) const
     {
         const double d = ((double)x - max) * per2, n = rint(d);
@@ -276,7 +276,7 @@ struct Entry {
 // What a cut is found with
 template <int NBINS>
 struct Search {
-    static constexpr int BINS = NBINS, LIST = NBINS / 4;
+    static constexpr int BINS = NBINS, LIST = 64;
     unsigned long long hist[BINS];
     Entry list[LIST];                                               // codes of the bin that a cut falls into
     float cut_x;
@@ -319,7 +319,7 @@ __device__ __forceinline__ void together()
 }
 template <int DT, bool STAGED, int W, int BINS>
 struct Draw {
-    static constexpr int NT = 64 * W, FEW = 40;
+    static constexpr int NT = 64 * W, FEW = 24;
     typedef Bins<BINS> B;
     Search<BINS> &s;
     unsigned long long *red;                                        // W each
@@ -374,6 +374,20 @@ struct Draw {
                 const uint64_t u = q(in[i] ? x[i] : (float)-INFINITY);
                 t += in[i] ? u : 0;
             }
+        }
+        return t;
+    }
+    // Sum of q(x) over all of the lane's codes; q(-inf) is 0
+    template <typename Q>
+    __device__ __forceinline__ uint64_t sum_all(Q q) const
+    {
+        uint64_t t = 0;
+        const int c1 = end;
+#pragma unroll 1
+        for (int c = begin + (threadIdx.x & 63) * 4; c < c1; c += 256) {
+            float x[4];
+            row.four(c, x);
+            t += (q(x[0]) + q(x[1])) + (q(x[2]) + q(x[3]));
         }
         return t;
     }
@@ -783,7 +797,7 @@ __device__ __forceinline__ void draw_row(const SampleArgs &a, int64_t n, typenam
     const Row row(mx, T, a.min(n), a.shift);
     uint64_t Z = 0;
     if (k <= 0 && P < 1.0) {
-        Z = d.total(d.sum([&](float v) { return row.units(v); }));
+        Z = d.total(d.sum_all([&](float v) { return row.units(v); }));
         // The codes further than D from the maximum have at most V (exp(-D / T) 2^shift + 1) units.  That much may be missing of (1 - P) Z, less
         // what rounding P Z and Z to f64 takes.
         const double spare = (1.0 - P) * (double)Z * 0.999 - (double)V - 4096.0;
