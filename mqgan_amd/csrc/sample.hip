@@ -855,7 +855,7 @@ template <int DT, int W>
 __global__ __launch_bounds__(64 * W, W == 8 ? 6 : 4) void sample_many_kernel(const SampleArgs a)
 {
     typedef Score<DT> S;
-    constexpr int KEPT = 256, QUADS = 4, LISTED = 128;              // LISTED: bins for a list's cuts
+    constexpr int KEPT = 256, QUADS = 4, LISTED = 256;              // LISTED: bins for a list's cuts
     typedef Few<DT, KEPT> F;
     extern __shared__ __attribute__((aligned(16))) char staged[];
     __shared__ Shared<W, 256> s;
@@ -970,7 +970,7 @@ static void sample_go(SampleArgs a, hipStream_t s)
 template <int DT, int W>
 static void sample_many(const SampleArgs &a, hipStream_t s)
 {
-    hipLaunchKernelGGL((sample_many_kernel<DT, W>), dim3((unsigned)((a.rows - a.row0 + W - 1) / W)), dim3(64 * W), std::max(row_bytes<DT>(a.V), W * sizeof(Search<128>)), s, a);
+    hipLaunchKernelGGL((sample_many_kernel<DT, W>), dim3((unsigned)((a.rows - a.row0 + W - 1) / W)), dim3(64 * W), std::max(row_bytes<DT>(a.V), W * sizeof(Search<256>)), s, a);
 }
 // Waves a row: fewer with more rows, whose waves fill the chip without barriers between them.  Measured (f32, normal scores with deviation 3;
 // us without a filter / top-p 0.95 / top-k 100 and top-p 0.95):
