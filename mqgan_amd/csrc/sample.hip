@@ -22,11 +22,10 @@
 // the bits of the score finds the cut instead.
 //
 // What bounds it: 16384 x 8192 f32 read once are 76 us at the 7.1 TB/s that loads alone reach here.  The maximum alone (temperature 0) takes 105 us,
-// top-k 20 147, top-k 100 with top-p 0.95 210: 70 % of the latter is the issue of vector instructions (6000 per row and wave slot), the rest
-// waits of the lists' waves.  Without top-k the masses of all codes are needed, 22 f64 operations each, twice for the one that is drawn: 16384 x
-// 8192 without a filter 280 us, top-p 0.95 530; 16384 x 1024 with top-p 0.9 65 (floor 9.5), 85 % of it vector issue.  Small calls are latency:
-// one row of 1000 codes with all filters 9 us, 48 of 8003 with top-p 0.95 26 us, a chain of some thirty dependent LDS accesses and barriers.
-// Selection by the bits of the scores over a row in memory took 2688 us where the lists take 210; a row in registers needs 215 of them.
+// top-k 20 145, top-k 100 with top-p 0.95 200: two thirds of the latter is the issue of vector instructions, the rest waits of the lists' waves.  Without top-k the masses of all codes are needed, 22 f64 operations each, twice for the one that is drawn: 16384 x
+// 8192 without a filter 280 us, top-p 0.95 530; 16384 x 1024 with top-p 0.9 60 (floor 9.5), of which reading and the first masses are 32, the cut
+// 20 and the draw 7.  Small calls are latency: one row of 1000 codes with all filters 9 us, 48 of 8003 with top-p 0.95 25 us, a chain of some thirty dependent LDS accesses and barriers.
+// Selection by the bits of the scores over a row in memory took 2688 us where the lists take 200; a row in registers needs 215 of them.
 #include <algorithm>
 
 #include "common.h"
@@ -849,7 +848,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 6 : W == 1 ? 5 : 4) void sample_ke
 
 // For many rows with top-k: a block takes W of them, one after the other as far as it needs the whole row - the next one is on its way
 // meanwhile - and what is done on a short list of codes is left to the end, where each wave has a row's.  Rows without such a list
-// come last, by the whole block.  One row a block and its list by one wave took 334 us where this takes 210 (16384 x 8192, top-k 100 and
+// come last, by the whole block.  One row a block and its list by one wave took 334 us where this takes 200 (16384 x 8192, top-k 100 and
 // top-p 0.95): the row's 32 KB of LDS were held while seven of eight waves had nothing to do.
 template <int DT, int W>
 __global__ __launch_bounds__(64 * W, W == 8 ? 6 : 4) void sample_many_kernel(const SampleArgs a)
