@@ -13,7 +13,7 @@
 // the unit counts as one unit (2^-49 at V = 8192) unless exp gives 0.
 //
 // Both cuts are a place in the order, (score, index): everything at or before it stays.  A block has one row, which is read once, into LDS, where
-// it fits (up to 14336 f32 or 16384 two-byte scores); each wave has a contiguous part, reads back what it wrote itself and needs no barrier
+// it fits (up to 9898 f32 or 14848 two-byte scores; past that each pass reads memory); each wave has a contiguous part, reads back what it wrote itself and needs no barrier
 // for that, and sums up to a code need one number per wave.  The codes that can be before a cut are found by a bound first - k of the threads'
 // own maxima are at least so large; codes beyond some distance hold less mass than top_p leaves out - and packed, in index order.
 // A cut is found without sorting: a histogram over the distance from the maximum (bins of equal RATIO, so neither the scores' scale nor masks of
@@ -21,11 +21,13 @@
 // are put into a list and counted against each other.  Where that list overflows (dozens of equal scores across the cut) radix selection over
 // the bits of the score finds the cut instead.
 //
-// What bounds it: 16384 x 8192 f32 read once are 76 us at the 7.1 TB/s that loads alone reach here.  The maximum alone (temperature 0) takes 105 us,
-// top-k 20 145, top-k 100 with top-p 0.95 200: two thirds of the latter is the issue of vector instructions, the rest waits of the lists' waves.  Without top-k the masses of all codes are needed, 22 f64 operations each, twice for the one that is drawn: 16384 x
-// 8192 without a filter 280 us, top-p 0.95 530; 16384 x 1024 with top-p 0.9 60 (floor 9.5), of which reading and the first masses are 32, the cut
-// 20 and the draw 7.  Small calls are latency: one row of 1000 codes with all filters 9 us, 48 of 8003 with top-p 0.95 25 us, a chain of some thirty dependent LDS accesses and barriers.
-// Selection by the bits of the scores over a row in memory took 2688 us where the lists take 200; a row in registers needs 215 of them.
+// What bounds it: 16384 x 8192 f32 read once are 76 us at the 7.1 TB/s that loads alone reach here.  The maximum alone (temperature 0) takes 105
+// us, top-k 20 145, top-k 100 with top-p 0.95 200: two thirds of the latter is the issue of vector instructions, the rest waits of the lists'
+// waves.  Without top-k the masses of all codes are needed, 22 f64 operations each: 16384 x 8192 without a filter 280 us, top-p 0.95 530; 16384 x
+// 1024 with top-p 0.9 60 (floor 9.5), of which reading and the first masses are 32, the cut 20 and the draw 7.  Small calls are latency, a chain
+// of some thirty dependent LDS accesses and barriers: one row of 1000 codes with all filters 9 us, 48 of 8003 with top-p 0.95 25, 64 of 32000 with
+// top-k 100 and top-p 0.9 27.  Selection by the bits of the scores over a row in memory took 2688 us where the lists take 200; a row in registers
+// needs 215 of them.
 #include <algorithm>
 
 #include "common.h"
@@ -45,7 +47,7 @@ struct SampleArgs {
     int64_t *idx;
     float *logp;
     int64_t row0, rows;                                              // those of a launch: [row0, rows)
-    int squeezes;                                                    // the rows' LDS has room for V indices
+    int squeezes;                                                    // there is a cut: the rows' LDS has room for V indices
     __device__ __forceinline__ double T(int64_t n) const { return temperature ? (double)temperature[n] : t0; }
     __device__ __forceinline__ double P(int64_t n) const { return top_p ? (double)top_p[n] : p0; }
     __device__ __forceinline__ double min(int64_t n) const { return min_p ? (double)min_p[n] : m0; }
@@ -287,7 +289,7 @@ struct Search {
 template <int DT, int KEPT>
 struct Few {
     alignas(16) typename Score<DT>::Raw x[KEPT];
-    uint16_t i[KEPT];                                               // a row in LDS has at most 16384
+    uint16_t i[KEPT];                                               // a row in LDS has at most 14848
     double T, P, min_p;
     int k, padded;
     float u;
@@ -326,13 +328,14 @@ struct Draw {
     View<DT, STAGED> row;
     float cut_x;                                                    // kept: at or before (cut_x, cut_i) in the order
     int cut_i;
-    int begin, end;
+    int begin, end, full;                                           // the wave's part; how many waves have a whole one, at least 1
 
     __device__ __forceinline__ Draw(Search<BINS> &s_, unsigned long long *red_, int *redi_, const View<DT, STAGED> &v) : s(s_), red(red_), redi(redi_), row(v), cut_x(-INFINITY), cut_i(-1)
     {                                                               // nothing with a score of -inf
         const int part = (row.n + 256 * W - 1) / (256 * W) * 256;
         begin = wave() * part;
         end = min(begin + part, row.n);
+        full = max(row.n / part, 1);
     }
     // The wave's part of the row: codes [begin, end), a multiple of 256 up to the last one's
     __device__ __forceinline__ int wave() const { return W > 1 ? (int)(threadIdx.x >> 6) : 0; }
@@ -637,6 +640,50 @@ struct Draw {
         }
         return many;
     }
+    // Puts the codes with x >= floor (> -inf) into x_ and index, in index order, where they are at most `room`.  How many they are.
+    __device__ __forceinline__ int gather(float floor, typename Score<DT>::Raw *x_, int *index, int room)
+    {
+        const int lane = threadIdx.x & 63;
+        int count = 0, at = 0, many = 0;
+#pragma unroll 1
+        for (int pass = 0; pass < 2; ++pass) {
+            for (int c = begin + lane * 4; c < begin + (end - begin + 255) / 256 * 256 + lane * 4; c += 256) {      // all lanes go round together
+                float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if (c < end) row.four(c, x);
+                uint64_t m[4];
+                int place = at;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    m[i] = __builtin_amdgcn_ballot_w64(x[i] >= floor);
+                    place += (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m[i] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m[i], 0u));
+                }
+                const int here = __popcll(m[0]) + __popcll(m[1]) + __popcll(m[2]) + __popcll(m[3]);
+                if (pass == 0) {
+                    count += here;
+                } else if (here) {
+                    at += here;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (x[i] >= floor) {
+                            x_[place] = Score<DT>::narrow(x[i]);
+                            index[place++] = c + i;
+                        }
+                }
+            }
+            if (pass) break;
+            if (lane == 0) redi[wave()] = count;
+            together<W>();
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                at += w < wave() ? redi[w] : 0;
+                many += redi[w];
+            }
+            if (many > room) return many;
+        }
+        if (threadIdx.x < (unsigned)(-many & 3)) x_[many + threadIdx.x] = Score<DT>::narrow(-INFINITY);      // to whole quads
+        together<W>();
+        return many;
+    }
     // Leaves the codes with x >= floor (> -inf) only, each wave in its part of the row: packed in index order, index[place] the code.  How many a
     // wave's are.
     __device__ __forceinline__ int squeeze(typename Score<DT>::Raw *x_, uint16_t *index, float floor)
@@ -683,10 +730,11 @@ __device__ __forceinline__ uint32_t values_above(const uint32_t (&key)[G], int n
     return t;
 }
 
-// The block's maximum, and a score that at least k codes reach where k <= 64 G W: k / W of each wave's own maxima do.  own: maxima of G groups
-// of the thread's codes.  Four groups cost 200 instructions more than one, so only a wave that has a whole row by itself takes them.
+// The block's maximum, and a score that at least `need` own maxima of each of the first `full` waves reach (the other waves' parts are shorter or
+// empty); need 0: none.  With need = k / full at least k codes reach it.  own: maxima of G groups of the thread's codes.  Four groups cost 200
+// instructions more than one, so only a wave that has a whole row by itself takes them.
 template <int W, int G>
-__device__ __forceinline__ float maximum(const float (&own)[G], int k, float *redf, int *redi, float *floor)
+__device__ __forceinline__ float maximum(const float (&own)[G], int need, int full, float *redf, int *redi, float *floor)
 {
     const int wave = W > 1 ? threadIdx.x >> 6 : 0;
     float most = own[0];
@@ -697,7 +745,7 @@ __device__ __forceinline__ float maximum(const float (&own)[G], int k, float *re
         key[g] = key_of(own[g]);
     }
     const float wmax = wave_max(most);
-    uint32_t low = k > 0 && k <= 64 * G * W ? values_above(key, (k + W - 1) / W) : 0;
+    uint32_t low = need ? (wave < full ? values_above(key, need) : 0xffffffffu) : 0;
     float mx = wmax;
     if (W > 1) {
         if ((threadIdx.x & 63) == 0) {
@@ -734,7 +782,9 @@ __device__ __forceinline__ int first_of(float mx, float own, const View<DT, STAG
     return (int)-block_max_f32<W>(-(float)first, redf);
 }
 
-// One row by a block of W waves.  HELD: it is read once, into LDS (at `lds`), each wave's part by itself; else each time from memory.  index:
+constexpr int LISTED = 6144;             // codes of a row that does not fit the LDS
+// One row by a block of W waves.  HELD: it is read once, into LDS (at `lds`), each wave's part by itself; else each time from memory, and what a
+// bound leaves of it goes into LDS (LISTED scores and their indices).  index:
 // NULL, or where V codes' indices may go, and few a list of the codes to keep.
 template <int DT, bool HELD, int W, typename H, int KEPT>
 __device__ __forceinline__ void draw_row(const SampleArgs &a, int64_t n, typename Score<DT>::Raw *lds, H &s, uint16_t *index, Few<DT, KEPT> *few)
@@ -774,7 +824,7 @@ __device__ __forceinline__ void draw_row(const SampleArgs &a, int64_t n, typenam
 #pragma unroll
     for (int g = 0; g < G; ++g) most = fmaxf(most, own[g]);
     float floor;
-    float mx = maximum<W, G>(own, HELD ? k : 0, s.redf, s.redi, &floor);
+    float mx = maximum<W, G>(own, k > 0 && k <= 64 * G * d.full ? (k + d.full - 1) / d.full : 0, d.full, s.redf, s.redi, &floor);
     if (mx == -INFINITY) {
         if (tid == 0) answer(-1, 0.f);
         return;
@@ -831,6 +881,15 @@ __device__ __forceinline__ void draw_row(const SampleArgs &a, int64_t n, typenam
             }
         }
     }
+    if (!HELD && floor > -INFINITY) {                               // the codes that a bound leaves, where they fit
+        int *which = reinterpret_cast<int *>(lds + LISTED);
+        const int many = d.gather(floor, lds, which, LISTED);
+        if (many <= LISTED) {
+            Draw<DT, true, W, H::BINS> l(s.search, s.red, s.counts, View<DT, true>{lds, many, false});
+            l.finish(row, mx, k, P, a.u[n], Z, [&](int c, float x, uint64_t mass) { answer(which[c], a.logp ? row.logp(x, mass) : 0.f); });
+            return;
+        }
+    }
     d.from_score(floor);
     d.finish(row, mx, k, P, a.u[n], Z, [&](int c, float x, uint64_t mass) { answer(squeezed ? index[c] : c, a.logp ? row.logp(x, mass) : 0.f); });
 }
@@ -854,7 +913,7 @@ template <int DT, int W>
 __global__ __launch_bounds__(64 * W, W == 8 ? 6 : 4) void sample_many_kernel(const SampleArgs a)
 {
     typedef Score<DT> S;
-    constexpr int KEPT = 256, QUADS = 4, LISTED = 256;              // LISTED: bins for a list's cuts
+    constexpr int KEPT = 256, QUADS = 4, BINS = 256;                // BINS: for a list's cuts
     typedef Few<DT, KEPT> F;
     extern __shared__ __attribute__((aligned(16))) char staged[];
     __shared__ Shared<W, 256> s;
@@ -894,10 +953,10 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 6 : 4) void sample_many_kernel(con
         }
     };
     load(0);
+    const int need = a.k0 > 0 && a.k0 <= 64 * d.full ? (a.k0 + d.full - 1) / d.full : 0;      // k is one for all rows here
     __syncthreads();
 #pragma unroll 1
     for (int r = 0; r < rows; ++r) {
-        const int k = few[r].k;
         const bool greedy = !(few[r].T > 0.0), padded = few[r].padded;
         float own[1] = {-INFINITY};                                 // the thread's maximum
 #pragma unroll
@@ -913,7 +972,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 6 : 4) void sample_many_kernel(con
         }
         if (r + 1 < rows && !few[r + 1].padded) load(r + 1);
         float floor;
-        const float mx = maximum<W, 1>(own, greedy ? 0 : k, s.redf, s.redi, &floor);
+        const float mx = maximum<W, 1>(own, greedy ? 0 : need, d.full, s.redf, s.redi, &floor);
         int state = F::DONE;
         if (padded || mx == -INFINITY) {
             if (tid == 0) answer(r, -1, 0.f);
@@ -936,8 +995,8 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 6 : 4) void sample_many_kernel(con
     if (wave < rows && few[wave].state >= 0) {
         const F &f = few[wave];
         const Row row(f.max, f.T, f.min_p, a.shift);
-        Search<LISTED> &there = reinterpret_cast<Search<LISTED> *>(staged)[wave];      // in the place of the rows
-        Draw<DT, true, 1, LISTED> l(there, s.red + wave, s.counts + wave, View<DT, true>{f.x, f.state, false});
+        Search<BINS> &there = reinterpret_cast<Search<BINS> *>(staged)[wave];      // in the place of the rows
+        Draw<DT, true, 1, BINS> l(there, s.red + wave, s.counts + wave, View<DT, true>{f.x, f.state, false});
         l.finish(row, f.max, f.k, f.P, f.u, 0, [&](int c, float x, uint64_t mass) { answer(wave, f.i[c], a.logp ? row.logp(x, mass) : 0.f); });
     }
 #pragma unroll 1
@@ -963,7 +1022,7 @@ template <int DT, int W>
 static void sample_go(SampleArgs a, hipStream_t s)
 {
     const size_t row = row_bytes<DT>(a.V), index = (size_t)a.V * sizeof(uint16_t);
-    a.squeezes = row + index <= ROOM && (a.top_k || a.k0 > 0 || a.top_p || a.p0 < 1.0);
+    a.squeezes = a.top_k || a.k0 > 0 || a.top_p || a.p0 < 1.0;
     hipLaunchKernelGGL((sample_kernel<DT, true, W>), dim3((unsigned)(a.rows - a.row0)), dim3(64 * W), row + (a.squeezes ? index : 0), s, a);
 }
 template <int DT, int W>
@@ -985,7 +1044,11 @@ static void sample_launch(const SampleArgs &a, hipStream_t s)
     const int64_t n = a.rows - a.row0;
     const int k = a.top_k ? 0 : a.k0;
     const bool greedy = !a.temperature && a.t0 == 0.0;
-    if (a.V > 16384 || row_bytes<DT>(a.V) > ROOM) hipLaunchKernelGGL((sample_kernel<DT, false, 8>), dim3((unsigned)n), dim3(512), 0, s, a);
+    if (row_bytes<DT>(a.V) + a.V * sizeof(uint16_t) > ROOM) {
+        const size_t room = LISTED * (sizeof(typename Score<DT>::Raw) + sizeof(int));
+        if (n <= 256) hipLaunchKernelGGL((sample_kernel<DT, false, 16>), dim3((unsigned)n), dim3(1024), room, s, a);
+        else hipLaunchKernelGGL((sample_kernel<DT, false, 8>), dim3((unsigned)n), dim3(512), room, s, a);
+    }
     else if (a.V <= 1024) n < 2048 ? sample_go<DT, 4>(a, s) : sample_go<DT, 1>(a, s);
     else if (a.V <= 4096) n <= 512 ? sample_go<DT, 8>(a, s) : n >= 4096 && a.V > 2048 && k > 0 && k <= 100 ? sample_many<DT, 4>(a, s) : sample_go<DT, 4>(a, s);
     else if (a.V <= 8192) n <= 256 && k <= 0 ? sample_go<DT, 16>(a, s) : n >= 4096 && (greedy || (k > 0 && k <= 128)) ? sample_many<DT, 8>(a, s) : sample_go<DT, 8>(a, s);
