@@ -7,8 +7,9 @@
 //
 // A row's statistics are an offset and a factor, p = factor * 2^(z log2 e - offset), and never one logarithm for both: a row of nothing but the
 // type's lowest value has log(sum) far under half an ulp of its maximum.  The offset is the maximum times log2 e, rounded; all of a row
-// uses the same, so its rounding goes into the factor.  Where that product could overflow (|maximum| > 1e37) the maximum itself is kept, as
-// a difference first: Offset.  A row of -inf alone has p = 0.  Padded rows are not read; their gradient is 0.
+// uses the same, so its rounding, which is half an ulp of the OFFSET in an exponent, goes into the factor.  That holds while half an ulp is far
+// under 1: at 2^20 it is 1/16, at 1e10 it would be 512 and every power 0 or infinite.  From 2^20 on the maximum itself is kept and z - maximum
+// taken first: Offset.  A row of -inf alone has p = 0.  Padded rows are not read; their gradient is 0.
 //
 // Scores are read once forward and once backward, which is the floor: 16384 x 8192 bf16, a fifth padded, 30 us at the 7.1 TB/s of loads alone and
 // 97 at the 4.97 TB/s of a copy.  Measured: rows 63 us, partial sums 12, loss 7; gradient 85 (non-temporal accesses: past the copy's rate).
@@ -41,15 +42,24 @@ constexpr float LOG2E = 1.44269504088896340736f;
 struct Offset {
     float o;                             // max log2 e, or the maximum itself where it is huge
     bool huge;
-    __device__ __forceinline__ explicit Offset(float m) : o(m == -INFINITY ? 0.f : m), huge(fabsf(o) > 1e37f) { o = huge ? o : o * LOG2E; }
+    __device__ __forceinline__ explicit Offset(float m) : o(m == -INFINITY ? 0.f : m), huge(fabsf(o) > 1048576.f)
+    {
+#pragma clang fp contract(off)
+        o = huge ? o : o * LOG2E;
+    }
     __device__ __forceinline__ Offset(float2 stats) : o(stats.x), huge(stats.y < 0.f) {}
     __device__ __forceinline__ float exp(float z) const { return __builtin_amdgcn_exp2f(huge ? (z - o) * LOG2E : fmaf(z, LOG2E, -o)); }
 };
-// what a sum over part of a row, whose maximum is m, counts for in the row's, whose maximum is M
+// What a sum over part of a row, whose maximum is m, counts for in the row's, whose maximum is M: the difference of the two offsets as the powers
+// took them, rounded once, also where only one of them is huge (maxima on both sides of 2^20 may be a fraction apart).  Not contracted: an FMA
+// of m, LOG2E and the other offset takes the exact product where the powers took the rounded one, half an ulp of the offset off.
 __device__ __forceinline__ float rebase(float m, float M)
 {
+#pragma clang fp contract(off)
     const Offset a(m), b(M);
-    return __builtin_amdgcn_exp2f(a.huge || b.huge ? (m - M) * LOG2E : a.o - b.o);
+    const float same = a.huge ? (a.o - b.o) * LOG2E : a.o - b.o;
+    const float mixed = a.huge ? fmaf(a.o, LOG2E, -b.o) : fmaf(-b.o, LOG2E, a.o);
+    return __builtin_amdgcn_exp2f(a.huge == b.huge ? same : mixed);
 }
 // (offset, factor); the factor is negative where the offset is the maximum itself
 __device__ __forceinline__ float2 stats_of(float m, float s)
