@@ -723,6 +723,11 @@ size_t mq_adamw_workspace(const int64_t *numel_host, int n);
 int mq_adamw_table_fill(const mqAdamwTensor *tensors_host, int n, int state_bits, void *table_host, size_t table_bytes);
 int mq_adamw_step(const mqAdamwDesc *desc_host, const int64_t *numel_host, const void *table, const void *const *grads_host,
                   const uint8_t *grad_types_host, void *control, void *workspace, size_t workspace_bytes, mqStream stream);
+/* The same where the device knows which tensors have a gradient (data-parallel ranks have to step the same ones): tensor i is left out
+ * where present[i] (device, n f32) is not above 0, as one without an address is.  The gradients of those count towards the norm: zeros. */
+int mq_adamw_step_present(const mqAdamwDesc *desc_host, const int64_t *numel_host, const void *table, const void *const *grads_host,
+                          const uint8_t *grad_types_host, const float *present, void *control, void *workspace, size_t workspace_bytes,
+                          mqStream stream);
 /* f32 moments to codes (to nearest) and back (f32, or bf16: exact in both), n a multiple of 256 */
 int mq_moments8_encode(const float *exp_avg, const float *exp_avg_sq, int64_t n, uint8_t *codes_avg, uint8_t *base_avg,
                        uint8_t *codes_avg_sq, uint8_t *base_avg_sq, mqStream stream);

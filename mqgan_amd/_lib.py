@@ -200,6 +200,7 @@ SIGNATURES = {
     "mq_adamw_workspace": (_Z, [_P, _I]),
     "mq_adamw_table_fill": (_I, [C.POINTER(AdamwTensor), _I, _I, _P, _Z]),
     "mq_adamw_step": (_I, [C.POINTER(AdamwDesc), _P, _P, _P, _P, _P, _P, _Z, _P]),
+    "mq_adamw_step_present": (_I, [C.POINTER(AdamwDesc), _P, _P, _P, _P, _P, _P, _P, _Z, _P]),
     "mq_moments8_encode": (_I, [_P, _P, _L, _P, _P, _P, _P, _P]),
     "mq_moments8_decode": (_I, [_P, _P, _P, _P, _L, _I, _P, _P, _P]),
     "mq_comm_unique_id": (_I, [_P]),

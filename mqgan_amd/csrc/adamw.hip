@@ -184,7 +184,7 @@ __global__ __launch_bounds__(256) void adamw_sumsq_kernel(const AwGrads grads, c
 // On the device because a captured step is replayed: count, bias corrections and random bits have to move on without the host.
 __global__ __launch_bounds__(1024) void adamw_prepare_kernel(const AwGrads grads, const AwRow *__restrict__ rows, int row0, int nrows, int first,
                                                              const double *__restrict__ part, int nparts, const AwHyper h,
-                                                             AwControl *__restrict__ ctl, AwState *__restrict__ st)
+                                                             const float *__restrict__ present, AwControl *__restrict__ ctl, AwState *__restrict__ st)
 {
     __shared__ double red[16];
     if (first) {
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(1024) void adamw_prepare_kernel(const AwGrads grads
         }
     }
     for (int i = threadIdx.x; i < nrows; i += 1024) {
-        if (!grads.g[i]) continue;
+        if (!grads.g[i] || (present && !(present[row0 + i] > 0.f))) continue;
         const int t = st[row0 + i].step + 1;
         const double lr = h.lr * (double)rows[row0 + i].lr_scale;
         AwState s;
@@ -340,14 +340,14 @@ __device__ __forceinline__ uint32_t nearest_add(float x) { return 0x7ffffu + ((m
 // which the hardware needs, so with eps = 0 an element that never had a gradient stays put instead of becoming 0 / 0.
 template <bool Q8>
 __global__ __launch_bounds__(256) void adamw_kernel(const AwGrads grads, const AwRow *__restrict__ rows, const int *__restrict__ row_of, int row0,
-                                                    int block0, const AwHyper h, const AwControl *__restrict__ ctl,
+                                                    int block0, const AwHyper h, const float *__restrict__ present, const AwControl *__restrict__ ctl,
                                                     const AwState *__restrict__ st)
 {
 #pragma clang fp contract(off)
     const int block = block0 + (int)(gridDim.x - 1 - blockIdx.x);
     const int r = row_of[block];
     const uint64_t tagged = grads.g[r - row0];
-    if (!tagged) return;                                            // no gradient this step: the tensor stays as it is
+    if (!tagged || (present && !(present[r] > 0.f))) return;        // no gradient this step: the tensor stays as it is
     const AwRow row = rows[r];
     const AwState s = st[r];
     const float coef = ctl->coef;
@@ -530,8 +530,8 @@ extern "C" int mq_adamw_table_fill(const mqAdamwTensor *tensors_host, int n, int
     return 0;
 }
 
-extern "C" int mq_adamw_step(const mqAdamwDesc *d, const int64_t *numel_host, const void *table, const void *const *grads_host,
-                             const uint8_t *grad_types_host, void *control, void *workspace, size_t workspace_bytes, mqStream stream)
+static int adamw_step(const mqAdamwDesc *d, const int64_t *numel_host, const void *table, const void *const *grads_host, const uint8_t *grad_types_host,
+                      const float *present, void *control, void *workspace, size_t workspace_bytes, mqStream stream)
 {
     MQ_REQUIRE(d && numel_host && table && grads_host && control, "mq_adamw_step: bad arguments");
     const int n = d->n_tensors;
@@ -573,20 +573,34 @@ extern "C" int mq_adamw_step(const mqAdamwDesc *d, const int64_t *numel_host, co
                 nb += (int)aw_blocks(numel_host[row0 + i]);
             }
             if (pass == 1)
-                hipLaunchKernelGGL(adamw_prepare_kernel, dim3(1), dim3(1024), 0, S(stream), g, rows, row0, nr, row0 == 0, part, parts, h, ctl, st);
+                hipLaunchKernelGGL(adamw_prepare_kernel, dim3(1), dim3(1024), 0, S(stream), g, rows, row0, nr, row0 == 0, part, parts, h, present, ctl, st);
             else if (nb && pass == 0) {
                 const int np = (int)cdiv(nb, AW_NORM);
                 hipLaunchKernelGGL(adamw_sumsq_kernel, dim3(np), dim3(256), 0, S(stream), g, rows, row_of, row0, block0, nb, parts, part);
                 parts += np;
             } else if (nb && d->state_bits == 8)
-                hipLaunchKernelGGL(adamw_kernel<true>, dim3(nb), dim3(256), 0, S(stream), g, rows, row_of, row0, block0, h, ctl, st);
+                hipLaunchKernelGGL(adamw_kernel<true>, dim3(nb), dim3(256), 0, S(stream), g, rows, row_of, row0, block0, h, present, ctl, st);
             else if (nb)
-                hipLaunchKernelGGL(adamw_kernel<false>, dim3(nb), dim3(256), 0, S(stream), g, rows, row_of, row0, block0, h, ctl, st);
+                hipLaunchKernelGGL(adamw_kernel<false>, dim3(nb), dim3(256), 0, S(stream), g, rows, row_of, row0, block0, h, present, ctl, st);
             block0 += nb;
         }
     }
     MQ_LAUNCH_CHECK("mq_adamw_step");
     return 0;
+}
+
+extern "C" int mq_adamw_step(const mqAdamwDesc *d, const int64_t *numel_host, const void *table, const void *const *grads_host,
+                             const uint8_t *grad_types_host, void *control, void *workspace, size_t workspace_bytes, mqStream stream)
+{
+    return adamw_step(d, numel_host, table, grads_host, grad_types_host, nullptr, control, workspace, workspace_bytes, stream);
+}
+
+extern "C" int mq_adamw_step_present(const mqAdamwDesc *d, const int64_t *numel_host, const void *table, const void *const *grads_host,
+                                     const uint8_t *grad_types_host, const float *present, void *control, void *workspace, size_t workspace_bytes,
+                                     mqStream stream)
+{
+    MQ_REQUIRE(present && (uintptr_t)present % 4 == 0, "mq_adamw_step_present: present is NULL or not aligned");
+    return adamw_step(d, numel_host, table, grads_host, grad_types_host, present, control, workspace, workspace_bytes, stream);
 }
 
 extern "C" int mq_moments8_encode(const float *exp_avg, const float *exp_avg_sq, int64_t n, uint8_t *codes_avg, uint8_t *base_avg,

@@ -70,8 +70,13 @@ class FlatArena:
                 p.data = view
                 p.grad = None if self.gather_mode else self.flat_grad[o:o + p.numel()].view_as(p)
         self._gathered = [False] * len(self.params)
+        # Which parameters got a gradient on some rank: device f32, one value each (above 0: yes), left by GradReducer.finish() for an
+        # optimiser that leaves out the others (track_presence); None: nothing was reduced, .grad tells.
+        self.track_presence = False
+        self.present = None
 
     def zero_grad(self):
+        self.present = None
         if self.gather_mode:
             for p in self.params:
                 p.grad = None
@@ -149,7 +154,10 @@ class FlatArena:
 class GradReducer:
     def __init__(self, arena: FlatArena, process_group=None, bucket_bytes: int = 32 << 20, average: bool = False, comm=None,
                  force: bool = False, tail_bytes: int = 1 << 20):
-        """``force``: hooks, per-bucket arena fill and asynchronous all-reduces even in a process group of ONE rank (the sum
+        """Buckets are launched in the order their gradients arrive, so with more than one of them backward has to reach the same
+        parameters on every rank; with one (models up to ``tail_bytes``) or a blocking ``comm`` the ranks may differ.
+
+        ``force``: hooks, per-bucket arena fill and asynchronous all-reduces even in a process group of ONE rank (the sum
         is then the identity) - lets a one-GPU box execute the production RCCL path end to end."""
         self.arena = arena
         self.pg = process_group
@@ -188,6 +196,7 @@ class GradReducer:
         self._launched = [False] * len(self.buckets)
         self._handles = []
         self._hooks = []
+        self._patterns = {}                    # which gradients were there -> that on the device: made once for every set met
         self._last_launch_event = None         # HIP event at the launch of the step's last bucket (while the StallClock runs)
         self._tail_pairs = []                  # (that event, event behind finish()'s waits) per step
         self.enabled = ((self.world > 1 or (force and dist.is_initialized())) and self.comm is None) if self._abi is None \
@@ -250,15 +259,7 @@ class GradReducer:
             ev = torch.cuda.Event(enable_timing=True)   # overwritten by every launch: what is left is the step's last one
             ev.record()
             self._last_launch_event = ev
-        if self._abi is not None:
-            self._handles.append(self._abi.all_reduce_async(self.arena.flat_grad[s:e]))
-            return
-        if self._drain_first:
-            torch.cuda.current_stream().synchronize()
-        if self._blocking:
-            dist.all_reduce(self.arena.flat_grad[s:e], op=dist.ReduceOp.SUM, group=self.pg)
-            return
-        self._handles.append(dist.all_reduce(self.arena.flat_grad[s:e], op=dist.ReduceOp.SUM, group=self.pg, async_op=True))
+        self._all_reduce(self.arena.flat_grad[s:e])
 
     def _on_grad(self, p):
         if not self.enabled:
@@ -268,13 +269,42 @@ class GradReducer:
         if self._pending[b] == 0 and not self._launched[b]:
             self._launch(b)
 
+    def _presence(self):
+        """This rank's part of ``arena.present``, to be summed; None where nobody asked or .grad is never None."""
+        arena = self.arena
+        if not (arena.track_presence and arena.gather_mode):
+            return None
+        pattern = tuple(p.grad is not None for p in arena.params)
+        if pattern not in self._patterns:
+            if len(self._patterns) >= 64:
+                self._patterns.clear()
+            self._patterns[pattern] = torch.tensor(pattern, dtype=torch.float32).to(arena.flat_grad.device)
+        arena.present = self._patterns[pattern].clone()
+        return arena.present
+
+    def _all_reduce(self, t):
+        """Sum over ranks: now (blocking), or from now on, waited for in finish()."""
+        if self._abi is not None:
+            self._handles.append(self._abi.all_reduce_async(t))
+            return
+        if self._drain_first:
+            torch.cuda.current_stream().synchronize()
+        if self._blocking:
+            dist.all_reduce(t, op=dist.ReduceOp.SUM, group=self.pg)
+            return
+        self._handles.append(dist.all_reduce(t, op=dist.ReduceOp.SUM, group=self.pg, async_op=True))
+
     def finish(self):
         """Call after backward: flush buckets that are still waiting (parameters without gradient),
-        wait for every collective.  The arena then holds SUMS over ranks; the 1 / world factor is
+        wait for every collective.  The arena then holds SUMS over ranks (and ``arena.present``, where an
+        optimiser asked for it, which parameters got a gradient anywhere); the 1 / world factor is
         applied inside the clip / Adam kernel (``grad_scale``) unless ``average`` asks for it here."""
         if self.comm is not None:
             self.arena.gather()
             self.comm.all_reduce_sum(self.arena.flat_grad)
+            present = self._presence()
+            if present is not None:
+                self.comm.all_reduce_sum(present)
             if self.average:
                 self.arena.flat_grad.mul_(1.0 / self.world)
             return
@@ -284,6 +314,9 @@ class GradReducer:
         for b in range(len(self.buckets)):
             if not self._launched[b]:
                 self._launch(b)
+        present = self._presence()
+        if present is not None:
+            self._all_reduce(present)
         for i, h in enumerate(self._handles):
             if self.clock is not None:
                 self.clock.bracket(h.wait)           # what the compute stream waits here was not hidden behind backward

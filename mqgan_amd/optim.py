@@ -25,10 +25,13 @@ class AdamW:
     ``state_bits``: 32, or 8 (two bytes a parameter plus two for every 256; see csrc/adamw.hip for the format).
     ``decays``: which tensors of an arena decay (a function of the parameter; default all).
     ``seed``: of the 8-bit moments' random rounding.  A tensor without a gradient is left out of a step, as in torch.optim.AdamW:
-    its moments and its step count stay."""
+    its moments and its step count stay.  Over an arena in gather mode whose gradients a ddp.GradReducer sums, that is a tensor without a
+    gradient on any rank, so that all ranks step the same ones (make the optimiser before the first step's ``finish()``)."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, seed=0, decays=None):
         self.arena = params if isinstance(params, FlatArena) else None
+        if self.arena is not None:
+            self.arena.track_presence = True
         groups = [{"params": params.params}] if self.arena is not None else list(params)
         if groups and not isinstance(groups[0], dict):
             groups = [{"params": groups}]
@@ -113,10 +116,13 @@ class AdamW:
     def _gradients(self, grads):
         if grads is not None:
             return grads
-        if self.arena is not None and self.arena.gather_mode:
-            self.arena.gather()                     # whatever the reducer has not moved yet; a parameter without gradient is left out
-            flat = self.arena.flat_grad
-            return [None if p.grad is None else flat[o:o + p.numel()] for p, o in zip(self.params, self.arena.offsets)]
+        arena = self.arena
+        if arena is not None and arena.gather_mode:
+            arena.gather()                          # whatever the reducer has not moved yet
+            # A parameter without gradient is left out.  Once a reducer has summed the arena over ranks, that is one without gradient on EVERY
+            # rank, which arena.present tells on the device: this rank's own .grad would have ranks step different tensors.
+            everywhere = arena.present is not None
+            return [arena.flat_grad[o:o + p.numel()] if everywhere or p.grad is not None else None for p, o in zip(self.params, arena.offsets)]
         return [p.grad for p in self.params]
 
     def step(self, max_norm=0.0, grad_scale=1.0, grads=None):
@@ -128,6 +134,7 @@ class AdamW:
         if not max_norm >= 0.0:
             raise ValueError(f"AdamW: max_norm {max_norm}")
         params = self.params
+        present = self.arena.present if self.arena is not None and grads is None else None
         grads = self._gradients(grads)
         if len(grads) != len(params):
             raise MqganHipError(f"AdamW: {len(grads)} gradients for {len(params)} parameters")
@@ -151,13 +158,16 @@ class AdamW:
                 if p.dtype != torch.float32 or not p.is_contiguous() or p.numel() != self._sizes[i] or p.device != self.device:
                     raise MqganHipError(f"AdamW: parameter {i} became {p.dtype} {tuple(p.shape)} on {p.device}")
             self._bind(at)
-        if torch.cuda.is_current_stream_capturing() and self._table is not (self._captured[-1] if self._captured else None):
-            self._captured.append(self._table)      # a graph reads it as long as it is replayed
+        if torch.cuda.is_current_stream_capturing():        # a graph reads them as long as it is replayed
+            self._captured += [x for x in (self._table, present) if x is not None and not any(x is y for y in self._captured)]
         d = self._desc
         d.lr, d.max_norm, d.grad_scale = float(self.lr), float(max_norm), float(grad_scale)
-        check(_lib.load().mq_adamw_step(C.byref(d), self._sizes, ptr(self._table), (C.c_void_p * len(params))(*addresses),
-                                        (C.c_uint8 * len(params)).from_buffer(types), ptr(self._control), ptr(self._workspace),
-                                        self._workspace.numel() * 8, stream()), "mq_adamw_step")
+        what = (C.byref(d), self._sizes, ptr(self._table), (C.c_void_p * len(params))(*addresses), (C.c_uint8 * len(params)).from_buffer(types))
+        where = (ptr(self._control), ptr(self._workspace), self._workspace.numel() * 8, stream())
+        if present is None:
+            check(_lib.load().mq_adamw_step(*what, *where), "mq_adamw_step")
+        else:
+            check(_lib.load().mq_adamw_step_present(*what, ptr(present), *where), "mq_adamw_step_present")
         self._scale = float(grad_scale)
 
     def grad_norm(self):
