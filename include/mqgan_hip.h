@@ -677,7 +677,8 @@ int mq_code_balance_bwd(const void *logits, int dtype, int64_t row_stride, const
  * first always; 1: all); min_p those with w >= min_p.  Drawn: the first in index order at which the running mass of the kept exceeds
  * uniform * (their mass).  temperature <= 0: the first of the order.  Scores of -inf and NaN are never drawn; a row of nothing else, and a
  * padded one, gives -1 (logp 0).  Where +inf occurs those codes share the draw evenly.  A uniform number outside [0, 1) is taken as the
- * nearest end.  The four settings come per row (device, f32 / int32) or, where that is NULL, from the descriptor.
+ * nearest end.  At most 2^19 codes: masses are whole numbers, all of a row's roundings together at most one step (2^-24) of the uniform numbers
+ * there, 2^-36 at 8192 codes.  The four settings come per row (device, f32 / int32) or, where that is NULL, from the descriptor.
  * idx (rows) int64; logp (rows) f32 or NULL: log of the drawn code's share of the kept mass. */
 typedef struct {
     int64_t rows, row_stride;

@@ -10,7 +10,9 @@
 // Masses are whole numbers: w rounded to units of 2^-min(51, 62 - ceil(log2 V)), exp in f64.  Their sums are exact whatever the order of
 // the additions, so histograms by atomics, scans and tree sums all agree to the last bit, and a cut or a draw next to a border falls the
 // same way on every run.  With f32 masses a row of 8192 codes would be drawn next to a border about once in 1000 rows.  A weight under
-// the unit counts as one unit (2^-49 at V = 8192) unless exp gives 0.
+// the unit counts as one unit (2^-49 at V = 8192) unless exp gives 0.  All roundings of a row together stay under V units of the largest weight: 2^-36
+// at 8192 codes, 2^-24 at 2^19, which is one step of the uniform numbers next to 1.  Past that whole units of codes that weigh nothing would be
+// drawn (at 2^20 by the three largest numbers under 1), so 2^19 codes is what a row may have.
 //
 // Both cuts are a place in the order, (score, index): everything at or before it stays.  A block has one row, which is read once, into LDS, where
 // it fits (up to 9898 f32 or 14848 two-byte scores; past that each pass reads memory); each wave has a contiguous part, reads back what it wrote itself and needs no barrier
@@ -1060,8 +1062,8 @@ extern "C" int mq_sample_codes(const mqSampleDesc *d, const void *logits, const 
 {
     MQ_REQUIRE(d && logits && uniform && idx, "mq_sample_codes: NULL argument");
     MQ_REQUIRE(d->dtype >= 0 && d->dtype <= 2, "mq_sample_codes: dtype %d (0 f32, 1 bf16, 2 f16)", d->dtype);
-    MQ_REQUIRE(d->rows > 0 && d->rows < INT32_MAX && d->codes > 0 && d->codes <= (1 << 20) && d->row_stride >= d->codes,
-               "mq_sample_codes: bad sizes (rows %lld, codes %d of at most 2^20, row stride %lld)", (long long)d->rows, d->codes, (long long)d->row_stride);
+    MQ_REQUIRE(d->rows > 0 && d->rows < INT32_MAX && d->codes > 0 && d->codes <= (1 << 19) && d->row_stride >= d->codes,
+               "mq_sample_codes: bad sizes (rows %lld, codes %d of at most 2^19, row stride %lld)", (long long)d->rows, d->codes, (long long)d->row_stride);
     MQ_REQUIRE(temperature || d->temperature >= 0.0, "mq_sample_codes: temperature %g", d->temperature);
     MQ_REQUIRE(top_k || d->top_k >= 0, "mq_sample_codes: top_k %d", d->top_k);
     MQ_REQUIRE(top_p || (d->top_p >= 0.0 && d->top_p <= 1.0), "mq_sample_codes: top_p %g is not in [0, 1]", d->top_p);

@@ -1639,7 +1639,7 @@ def sample_codes(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, t
     w >= min_p; drawn is the first code, in index order, at which the running mass exceeds uniform times the mass of all kept ones.
     temperature 0: the largest score, lowest index.  Each setting is a number or a tensor with one value per row.  Scores of -inf and NaN
     are never drawn; a row of nothing else, and a ``padded`` one (uint8 / bool, 1 = padded), gives -1.  Masses are exact whole numbers
-    (csrc/sample.hip): the same inputs draw the same codes on every run."""
+    (csrc/sample.hip): the same inputs draw the same codes on every run; V is at most 2^19."""
     z, kind, rows, V, stride = _score_rows(logits, "sample_codes")
     shape = logits.shape[:-1]
     if uniform.dtype != F32 or uniform.numel() != rows:
