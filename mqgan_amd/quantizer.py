@@ -172,15 +172,16 @@ class L2Quantizer(nn.Module):
         return x + (codes - x).detach(), idx
 
     def scores(self, x: torch.Tensor, temperature: float = 1.0) -> torch.Tensor:
-        """-|x - c|^2 / temperature for every code, up to a term of the vector alone: (..., d) -> (..., codebook_size) f32.  The gradient
-        goes to x (the codebook moves by its EMA)."""
+        """-|x - c|^2 / temperature for every code, up to a term of the vector alone: (..., d) -> (..., codebook_size) f32, on exact f32 products
+        whatever the layers' precision, as ``indices``: with vectors rounded to bf16 the scores are off by 2^-8 |x| |c| / temperature, more than
+        lies between codes.  The gradient goes to x (the codebook moves by its EMA)."""
         if not temperature > 0:
             raise ValueError(f"L2Quantizer.scores: temperature {temperature}")
         with torch.no_grad():
             w, wt = ops.weight_prep(ops.scale(self.codebook, 2.0 / temperature), None, need_crsk=x.requires_grad)
             bias = ops.scale(ops.l2_codebook_norms(self.codebook), -1.0 / temperature)
         rows = x.numel() // self.dim
-        d = ops.conv_desc(1, 1, rows, self.dim, self.codebook_size, 1, 1)
+        d = ops.conv_desc(1, 1, rows, self.dim, self.codebook_size, 1, 1, precision="f32")
         y = ops.conv(x.reshape(1, 1, rows, self.dim).contiguous(), w, wt, bias, d, out_f32=True)
         return ops.to_f32(y).view(*x.shape[:-1], self.codebook_size)
 
