@@ -35,15 +35,18 @@ class AdamW:
         groups = [{"params": params.params}] if self.arena is not None else list(params)
         if groups and not isinstance(groups[0], dict):
             groups = [{"params": groups}]
-        self.params, self.weight_decays, self.lr_scales = [], [], []
+        self.params, self.weight_decays, self.lr_scales, self.groups = [], [], [], []        # groups: positions of what shares a decay and a scale
         for g in groups:
             unknown = set(g) - {"params", "weight_decay", "lr_scale"}
             if unknown:
                 raise ValueError(f"AdamW: a group has params, weight_decay and lr_scale, not {sorted(unknown)}")
+            mine = {}
             for p in g["params"]:
+                mine.setdefault(decays is None or bool(decays(p)), []).append(len(self.params))
                 self.params.append(p)
                 self.weight_decays.append(float(g.get("weight_decay", weight_decay)) if decays is None or decays(p) else 0.0)
                 self.lr_scales.append(float(g.get("lr_scale", 1.0)))
+            self.groups += [mine[k] for k in (True, False) if k in mine]
         if not self.params:
             raise ValueError("AdamW: no parameters")
         if len({id(p) for p in self.params}) != len(self.params):
@@ -220,8 +223,9 @@ class AdamW:
         return max(self._steps()[0])
 
     def state_dict(self):
-        """torch.optim.AdamW's format (moments in f32), so a state moves between the two and between 8 and 32 bits; for 8 bits the codes
-        besides, from which a run goes on bit for bit."""
+        """torch.optim.AdamW's format (moments in f32): one parameter group for every group given, and for the tensors of one that ``decays``
+        leaves out, each with its own lr and weight decay.  A torch.optim.AdamW over the same groups takes it, and 8 and 32 bits take each
+        other's; for 8 bits it has the codes and the seed besides, from which a run goes on bit for bit."""
         steps, calls = self._steps()
         m, v = self.moments()
         state = {}
@@ -229,21 +233,33 @@ class AdamW:
             if t:
                 state[i] = {"step": torch.tensor(float(t)), "exp_avg": m[at:at + p.numel()].view_as(p).clone(),
                             "exp_avg_sq": v[at:at + p.numel()].view_as(p).clone()}
-        group = {"lr": self.lr, "betas": self.betas, "eps": self.eps, "weight_decay": max(self.weight_decays), "amsgrad": False,
-                 "maximize": False, "foreach": None, "capturable": False, "differentiable": False, "fused": None,
-                 "initial_lr": self.base_lr, "params": list(range(len(self.params)))}
-        sd = {"state": state, "param_groups": [group], "mqgan_amd_calls": calls}
+        groups = [{"lr": self.lr * self.lr_scales[g[0]], "betas": self.betas, "eps": self.eps, "weight_decay": self.weight_decays[g[0]],
+                   "amsgrad": False, "maximize": False, "foreach": None, "capturable": False, "differentiable": False, "fused": None,
+                   "decoupled_weight_decay": True, "initial_lr": self.base_lr * self.lr_scales[g[0]], "lr_scale": self.lr_scales[g[0]],
+                   "params": list(g)} for g in self.groups]
+        sd = {"state": state, "param_groups": groups, "mqgan_amd_calls": calls, "mqgan_amd_lr": self.lr}
         if self.state_bits == 8:
             sd["mqgan_amd_moments8"] = {"codes": (self.exp_avg.clone(), self.exp_avg_sq.clone()), "bases": tuple(b.clone() for b in self._bases),
-                                        "sizes": list(self._sizes)}
+                                        "sizes": list(self._sizes), "seed": self.seed}
         return sd
 
     def load_state_dict(self, sd):
+        """A state of this class or of torch.optim.AdamW (or Adam, train.FlatAdam).  Where its groups are this optimiser's - the same
+        tensors for a state of this class, the same numbers of them otherwise - lr, scales, weight decays, betas and eps come with it, as in
+        torch; where they are not, lr alone (the first group's) does and the tensors go by their position."""
+        own = "mqgan_amd_calls" in sd
+        saved = sd.get("param_groups") or []
+        ids = [[int(i) for i in g["params"]] for g in saved]
+        if own:
+            fits = ids == self.groups and "mqgan_amd_lr" in sd           # without: one group for all, as this class wrote them at first
+        else:
+            fits = [len(g) for g in ids] == [len(g) for g in self.groups]
+        place = dict(zip((i for g in ids for i in g), (i for g in self.groups for i in g))) if fits else {}
         steps = [0] * len(self.params)
         total = self.exp_avg.numel()
         m, v = (torch.zeros(total, dtype=torch.float32, device=self.device) for _ in range(2))
         for i, st in sd.get("state", {}).items():
-            i = int(i)
+            i = place.get(int(i), int(i))
             if i >= len(self.params) or st["exp_avg"].numel() != self._sizes[i]:
                 raise MqganHipError(f"AdamW: the state's entry {i} does not fit the parameters")
             at = self.positions[i]
@@ -251,11 +267,47 @@ class AdamW:
             v[at:at + self._sizes[i]].copy_(st["exp_avg_sq"].reshape(-1))
             steps[i] = int(float(st["step"]))
         held = sd.get("mqgan_amd_moments8")
-        if self.state_bits == 8 and held is not None and list(held["sizes"]) == list(self._sizes):
-            for mine, theirs in zip((self.exp_avg, self.exp_avg_sq) + self._bases, tuple(held["codes"]) + tuple(held["bases"])):
-                mine.copy_(theirs)
+        held = held if self.state_bits == 8 and held is not None and list(held["sizes"]) == list(self._sizes) else None
+        mine = (self.exp_avg, self.exp_avg_sq) + (self._bases or ())
+        theirs = tuple(held["codes"]) + tuple(held["bases"]) if held else ()
+        if any(a.shape != b.shape or a.dtype != b.dtype for a, b in zip(mine, theirs)):
+            raise MqganHipError("AdamW: the state's 8-bit moments do not fit the parameters")
+        self._load_groups(saved, fits, sd.get("mqgan_amd_lr"))
+        if held:
+            for a, b in zip(mine, theirs):
+                a.copy_(b)
+            self.seed = int(held.get("seed", self.seed))
+            self._desc.seed = self.seed & (2 ** 64 - 1)
         else:
             self.load_moments(m, v)
         self._set_steps(steps, int(sd.get("mqgan_amd_calls", max(steps))))
-        if sd.get("param_groups"):
-            self.lr = sd["param_groups"][0].get("lr", self.lr)
+
+    def _load_groups(self, saved, fits, lr):
+        """lr and, where the groups are this optimiser's, the rest of their settings."""
+        if not saved:
+            return
+        if any(g.get("amsgrad") or g.get("maximize") for g in saved):
+            raise MqganHipError("AdamW: the state is of an optimiser with amsgrad or maximize, which this one has not")
+        lrs = [float(g.get("lr", self.lr)) for g in saved]
+        if not fits:
+            self.lr = lrs[0] if lr is None else float(lr)
+            return
+        betas, eps = ([tuple(float(b) for b in g.get("betas", self.betas)) for g in saved], [float(g.get("eps", self.eps)) for g in saved])
+        if len(set(betas)) > 1 or len(set(eps)) > 1:
+            raise MqganHipError("AdamW: the state's groups differ in betas or eps, which are one for all of this optimiser's")
+        scales = [g.get("lr_scale") for g in saved]
+        if lr is None or None in scales:                # not of this class: the first group's scale as it is here, the others' by their lr
+            mine = [self.lr_scales[g[0]] for g in self.groups]
+            lr = lrs[0] / mine[0] if mine[0] > 0 and lrs[0] > 0 else max(lrs)
+            scales = [x / lr for x in lrs] if lr > 0 else mine
+        self.lr = float(lr)
+        self.betas, self.eps = betas[0], eps[0]
+        d = self._desc
+        d.beta1, d.beta2, d.eps = self.betas[0], self.betas[1], self.eps
+        before = self.weight_decays, self.lr_scales
+        self.weight_decays, self.lr_scales = list(before[0]), list(before[1])
+        for group, g, scale in zip(self.groups, saved, scales):
+            for i in group:
+                self.weight_decays[i], self.lr_scales[i] = float(g.get("weight_decay", before[0][i])), float(scale)
+        if (self.weight_decays, self.lr_scales) != before:
+            self._bind(self._addresses)                 # both stand in the table
