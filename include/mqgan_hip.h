@@ -699,7 +699,8 @@ int mq_sample_codes(const mqSampleDesc *desc_host, const void *logits, const flo
  * has a sign and 7 bits of c (126 infinite, 127 NaN), v 8 bits (254, 255).  Rounded stochastically with a hash of (seed, call, position).
  *   table_fill   host: checks the tensors and lays out what the step reads, into table_host (table_bytes()); the caller copies it to the
  *                device.  It holds addresses: fill it again when a tensor moves.
- *   control      control_bytes(n) device bytes, zeroed by the caller once: the norm's square (f64 at byte 0), the calls so far (int64 at 8),
+ *   control      control_bytes(n) device bytes, zeroed by the caller once: the norm's square (f64 at byte 0) and the |grad_scale| of
+ *                the call it is of (f64 at 32; both stay through calls with max_norm 0), the calls so far (int64 at 8),
  *                and from byte 64 on 16 bytes per tensor whose first int32 is the tensor's step count t
  *   workspace    device bytes for the norm's partial sums; one step at a time may use control and workspace
  *   step         grads_host: n device addresses, NULL = no gradient (that tensor, its moments and its step count stay as they are);

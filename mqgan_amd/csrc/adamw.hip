@@ -43,7 +43,9 @@ struct AwControl {                    // start of the control buffer; AwState pe
     int64_t calls;
     float coef;
     uint32_t k0, k1;
-    uint32_t pad[9];
+    uint32_t pad0;
+    double norm_scale;                // |grad_scale| of the call that sumsq is of
+    uint32_t pad[6];
 };
 struct AwState {
     int step;
@@ -201,6 +203,7 @@ __global__ __launch_bounds__(1024) void adamw_prepare_kernel(const AwGrads grads
                 const double c = h.max_norm / (sqrt(t) * fabs(h.grad_scale) + 1e-6);
                 coef = c < 1.0 ? c * h.grad_scale : (c >= 1.0 ? h.grad_scale : c);    // a NaN norm makes the step NaN, as the formula says
                 ctl->sumsq = t;
+                ctl->norm_scale = fabs(h.grad_scale);
             }
             ctl->coef = (float)coef;
             const int64_t calls = ctl->calls + 1;

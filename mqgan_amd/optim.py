@@ -84,7 +84,6 @@ class AdamW:
         self._workspace = new(lib.mq_adamw_workspace(self._sizes, n) // 8, torch.float64)
         self._desc = AdamwDesc(n_tensors=n, state_bits=state_bits, beta1=self.betas[0], beta2=self.betas[1], eps=self.eps, seed=self.seed & (2 ** 64 - 1))
         self._addresses, self._captured = None, []
-        self._scale = 1.0
         self._bind([p.data_ptr() for p in self.params])
 
     # -- tables ---------------------------------------------------------------------------------
@@ -171,11 +170,11 @@ class AdamW:
             check(_lib.load().mq_adamw_step(*what, *where), "mq_adamw_step")
         else:
             check(_lib.load().mq_adamw_step_present(*what, ptr(present), *where), "mq_adamw_step_present")
-        self._scale = float(grad_scale)
 
     def grad_norm(self):
         """Norm of the scaled gradients before clipping, of the last step with ``max_norm`` > 0 (device scalar; reading it synchronises)."""
-        return self._control[:1].view(torch.float64).sqrt()[0].float() * abs(self._scale)
+        f = self._control.view(torch.float64)
+        return (f[0].sqrt() * f[4]).float()             # on the device both, so it is right after a replay too
 
     # -- moments and state ------------------------------------------------------------------------
     def moments(self, dtype=torch.float32):
