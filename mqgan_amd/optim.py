@@ -76,7 +76,7 @@ class AdamW:
             self.exp_avg, self.exp_avg_sq = new(total, torch.uint8), new(total, torch.uint8)
             self._bases = new(total // GROUP, torch.uint8), new(total // GROUP, torch.uint8)
         lib = _lib.load()
-        self._sizes = (C.c_int64 * n)(*sizes)
+        self._sizes, self._shapes = (C.c_int64 * n)(*sizes), [p.shape for p in self.params]
         self._table_bytes = lib.mq_adamw_table_bytes(self._sizes, n)
         if not self._table_bytes:
             raise MqganHipError("AdamW: too many elements")
@@ -127,10 +127,15 @@ class AdamW:
             return [arena.flat_grad[o:o + p.numel()] if everywhere or p.grad is not None else None for p, o in zip(self.params, arena.offsets)]
         return [p.grad for p in self.params]
 
+    def _lies_like(self, g, i):
+        """Whether a gradient that has not the shape its parameter was given with holds the same elements in the same order: a flat one, as an
+        arena's, or one of the shape that the parameter has by now."""
+        return g.numel() == self._sizes[i] and (g.dim() == 1 or g.shape == self.params[i].shape)
+
     def step(self, max_norm=0.0, grad_scale=1.0, grads=None):
         """``max_norm`` > 0: clip the norm of all gradients to it (``grad_norm()`` then has the norm).  ``grad_scale``: factor on every
         gradient (1 / world size for summed ones).  ``grads``: the gradients (f32, bf16 or f16; None = none) in the order of the
-        parameters, instead of their ``.grad``."""
+        parameters, each of its parameter's shape or flat, instead of their ``.grad``."""
         if torch.cuda.current_device() != self.device.index:
             raise MqganHipError(f"AdamW: the parameters live on {self.device} but the current HIP device is cuda:{torch.cuda.current_device()}")
         if not max_norm >= 0.0:
@@ -140,13 +145,13 @@ class AdamW:
         grads = self._gradients(grads)
         if len(grads) != len(params):
             raise MqganHipError(f"AdamW: {len(grads)} gradients for {len(params)} parameters")
-        held, addresses, types = [], [], bytearray(len(params))
-        for i, (g, size) in enumerate(zip(grads, self._sizes)):
+        held, addresses, types, device = [], [], bytearray(len(params)), self.device.index
+        for i, (g, shape) in enumerate(zip(grads, self._shapes)):
             if g is None:
                 addresses.append(0)
                 continue
             t = _GRAD_TYPES.get(g.dtype)
-            if t is None or g.numel() != size or g.device != self.device:
+            if t is None or g.get_device() != device or (g.shape != shape and not self._lies_like(g, i)):
                 raise MqganHipError(f"AdamW: gradient {i} is {g.dtype} {tuple(g.shape)} on {g.device}; its parameter is {tuple(params[i].shape)} "
                                     f"on {self.device}")
             if not g.is_contiguous():
