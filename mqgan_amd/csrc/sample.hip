@@ -15,7 +15,7 @@
 // drawn (at 2^20 by the three largest numbers under 1), so 2^19 codes is what a row may have.
 //
 // Both cuts are a place in the order, (score, index): everything at or before it stays.  A block has one row, which is read once, into LDS, where
-// it fits (up to 9898 f32 or 14848 two-byte scores; past that each pass reads memory); each wave has a contiguous part, reads back what it wrote itself and needs no barrier
+// it fits (up to 9896 f32 or 14848 two-byte scores; past that each pass reads memory); each wave has a contiguous part, reads back what it wrote itself and needs no barrier
 // for that, and sums up to a code need one number per wave.  The codes that can be before a cut are found by a bound first - k of the threads'
 // own maxima are at least so large; codes beyond some distance hold less mass than top_p leaves out - and packed, in index order.
 // A cut is found without sorting: a histogram over the distance from the maximum (bins of equal RATIO, so neither the scores' scale nor masks of
