@@ -308,10 +308,16 @@ def check(rc, what=""):
         raise MqganHipError(f"{what}: {msg}" if what else msg)
 
 
+# torch's own shortcut to the stream's handle, 4 us less a call than through a Stream object; not a documented function, so it may be missing
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream():
     """HIP stream every kernel of this call is launched on: the current stream of the CURRENT device.  ptr() refuses
     tensors that live on another device, so a launch can never pair device-N pointers with device-0's stream."""
-    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))      # without the Stream object: 4 us less a call
+    if _raw_stream is None:
+        return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    return C.c_void_p(_raw_stream(torch.cuda.current_device()))
 
 
 def ptr(t, dtype=None, allow_none=False):
