@@ -1657,6 +1657,8 @@ def sample_codes(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, t
             if dtype == torch.int32 and v.dtype != dtype:
                 v = v.clamp(-1, V)                  # before 32 bits would wrap it
             held[name] = v.reshape(-1).to(dtype).contiguous()
+            if name == "temperature" and v.dtype == torch.float64:       # above 0 stays above 0: 0 is another rule where scores tie
+                held[name] = torch.where(v.reshape(-1) > 0, held[name].clamp(min=2.0 ** -149), held[name])
             return held[name]
         t, k = setting("temperature", temperature, F32), setting("top_k", top_k, torch.int32)
         p, m = setting("top_p", top_p, F32), setting("min_p", min_p, F32)

@@ -45,3 +45,14 @@ def test_wider_rows_are_refused():
     from mqgan_amd._lib import MqganHipError
     with pytest.raises(MqganHipError, match="2\\^19"):
         ops.sample_codes(torch.zeros(1, MOST + 1, device=DEV), torch.zeros(1, device=DEV))
+
+
+def test_a_temperature_under_the_range_of_f32_is_not_zero():
+    """Equal largest scores share the draw at every temperature above 0; at 0 the first of them has it."""
+    from mqgan_amd import ops
+    z = torch.zeros(4, 3, device=DEV)
+    z[:, 0] = -1.0
+    t = torch.tensor([1e-50, 1e-300, 0.0, -1e-50], dtype=torch.float64, device=DEV)
+    u = torch.full((4,), 0.9, device=DEV)
+    assert ops.sample_codes(z, u, temperature=t).tolist() == [2, 2, 1, 1]
+    assert ops.sample_codes(z, u, temperature=1e-50).tolist() == [2] * 4
