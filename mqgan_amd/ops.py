@@ -1624,16 +1624,23 @@ def _score_ptr(z):
     return C.c_void_p(z.data_ptr())
 
 
-def _row_mask(padded, rows, like, what):
+def _one_a_row(t, lead):
+    """Whether t has a value for each row of scores of leading shape ``lead``, in the rows' order: of that shape, up to dimensions of 1, or flat."""
+    if t.shape == lead:
+        return True
+    return t.numel() == lead.numel() and (t.dim() == 1 or [n for n in t.shape if n != 1] == [n for n in lead if n != 1])
+
+
+def _row_mask(padded, rows, lead, what):
     if padded is None:
         return None
-    if padded.dtype not in (torch.uint8, torch.bool) or padded.numel() != rows:
+    if padded.dtype not in (torch.uint8, torch.bool) or not _one_a_row(padded, lead):
         raise _lib.MqganHipError(f"{what}: padded is uint8 or bool with one value per row ({rows}), got {padded.dtype} {tuple(padded.shape)}")
     return padded.contiguous()                      # a bool is a byte of 0 or 1
 
 
 def sample_codes(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, padded=None, return_logp=False):
-    """Draw a code per row: logits (..., V) f32 / bf16 / f16, ``uniform`` (...) f32 in [0, 1) -> int64 codes (...) [, f32 log of the drawn
+    """Draw a code per row: logits (..., V) f32 / bf16 / f16, ``uniform`` (...) or flat, f32 in [0, 1) -> int64 codes (...) [, f32 log of the drawn
     code's share of what was kept].  The codes in order of (score descending, index ascending), w = exp((z - max) / temperature): ``top_k``
     keeps the first k (0: all), ``top_p`` every code before which less than top_p of their mass lies (1: all), ``min_p`` those with
     w >= min_p; drawn is the first code, in index order, at which the running mass exceeds uniform times the mass of all kept ones.
@@ -1642,7 +1649,7 @@ def sample_codes(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, t
     (csrc/sample.hip): the same inputs draw the same codes on every run; V is at most 2^19."""
     z, kind, rows, V, stride = _score_rows(logits, "sample_codes")
     shape = logits.shape[:-1]
-    if uniform.dtype != F32 or uniform.numel() != rows:
+    if uniform.dtype != F32 or not _one_a_row(uniform, shape):
         raise _lib.MqganHipError(f"sample_codes: one f32 uniform number per row ({rows}), got {uniform.dtype} {tuple(uniform.shape)}")
     idx = torch.empty(shape, dtype=torch.int64, device=z.device)
     logp = _empty(shape, z) if return_logp else None
@@ -1652,7 +1659,7 @@ def sample_codes(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, t
         def setting(name, v, dtype):
             if not isinstance(v, torch.Tensor):
                 return None
-            if v.numel() != rows:
+            if not _one_a_row(v, shape):
                 raise _lib.MqganHipError(f"sample_codes: {name} is a number or has one value per row ({rows}), got {tuple(v.shape)}")
             if dtype == torch.int32 and v.dtype != dtype:
                 v = v.clamp(-1, V)                  # before 32 bits would wrap it
@@ -1662,7 +1669,7 @@ def sample_codes(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, t
             return held[name]
         t, k = setting("temperature", temperature, F32), setting("top_k", top_k, torch.int32)
         p, m = setting("top_p", top_p, F32), setting("min_p", min_p, F32)
-        mask, u = _row_mask(padded, rows, z, "sample_codes"), uniform.reshape(-1).contiguous()
+        mask, u = _row_mask(padded, rows, shape, "sample_codes"), uniform.reshape(-1).contiguous()
         d = _lib.SampleDesc(rows, stride, V, kind, 0.0 if t is not None else float(temperature), 0.0 if p is not None else float(top_p),
                             0.0 if m is not None else float(min_p), 0 if k is not None else min(int(top_k), V))
         check(L().mq_sample_codes(C.byref(d), _score_ptr(z), fptr(u), fptr(t, True), ptr(k, torch.int32, True), fptr(p, True), fptr(m, True),
@@ -1683,7 +1690,7 @@ class CodeBalanceFn(torch.autograd.Function):
                                      f"{idx.dtype} {tuple(idx.shape)}")
         if K == 0:
             raise _lib.MqganHipError("code_balance_loss: no assignments")
-        mask = _row_mask(padded, rows, z, "code_balance_loss")
+        mask = _row_mask(padded, rows, lead, "code_balance_loss")
         lib = L()
         n_stats, n_sums = 2 * rows + (rows & 1) * 2, (2 * V + 4) // 4 * 4
         nbytes = lib.mq_code_balance_workspace(rows, V, kind)
