@@ -1626,9 +1626,7 @@ def _score_ptr(z):
 
 def _one_a_row(t, lead):
     """Whether t has a value for each row of scores of leading shape ``lead``, in the rows' order: of that shape, up to dimensions of 1, or flat."""
-    if t.shape == lead:
-        return True
-    return t.numel() == lead.numel() and (t.dim() == 1 or [n for n in t.shape if n != 1] == [n for n in lead if n != 1])
+    return t.shape == lead or (t.numel() == lead.numel() and (t.dim() == 1 or [n for n in t.shape if n != 1] == [n for n in lead if n != 1]))
 
 
 def _row_mask(padded, rows, lead, what):

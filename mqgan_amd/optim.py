@@ -127,11 +127,6 @@ class AdamW:
             return [arena.flat_grad[o:o + p.numel()] if everywhere or p.grad is not None else None for p, o in zip(self.params, arena.offsets)]
         return [p.grad for p in self.params]
 
-    def _lies_like(self, g, i):
-        """Whether a gradient that has not the shape its parameter was given with holds the same elements in the same order: a flat one, as an
-        arena's, or one of the shape that the parameter has by now."""
-        return g.numel() == self._sizes[i] and (g.dim() == 1 or g.shape == self.params[i].shape)
-
     def step(self, max_norm=0.0, grad_scale=1.0, grads=None):
         """``max_norm`` > 0: clip the norm of all gradients to it (``grad_norm()`` then has the norm).  ``grad_scale``: factor on every
         gradient (1 / world size for summed ones).  ``grads``: the gradients (f32, bf16 or f16; None = none) in the order of the
@@ -146,12 +141,13 @@ class AdamW:
         if len(grads) != len(params):
             raise MqganHipError(f"AdamW: {len(grads)} gradients for {len(params)} parameters")
         held, addresses, types, device = [], [], bytearray(len(params)), self.device.index
-        for i, (g, shape) in enumerate(zip(grads, self._shapes)):
+        for i, (g, shape, size) in enumerate(zip(grads, self._shapes, self._sizes)):
             if g is None:
                 addresses.append(0)
                 continue
             t = _GRAD_TYPES.get(g.dtype)
-            if t is None or g.get_device() != device or (g.shape != shape and not self._lies_like(g, i)):
+            # of its parameter's shape as it was given, or as it is by now, or flat (an arena's): the same elements in the same order
+            if t is None or g.get_device() != device or (g.shape != shape and (g.numel() != size or (g.dim() != 1 and g.shape != params[i].shape))):
                 raise MqganHipError(f"AdamW: gradient {i} is {g.dtype} {tuple(g.shape)} on {g.device}; its parameter is {tuple(params[i].shape)} "
                                     f"on {self.device}")
             if not g.is_contiguous():
