@@ -11,11 +11,16 @@
 // under 1: at 2^20 it is 1/16, at 1e10 it would be 512 and every power 0 or infinite.  From 2^20 on the maximum itself is kept and z - maximum
 // taken first: Offset.  A row of -inf alone has p = 0.  Padded rows are not read; their gradient is 0.
 //
+// Sums: a row's in f32, lane by lane and then as a tree; P's over rows in f32 within a team (a lane adds one row after the other, 16384 rows of 8192
+// codes 32 of them, of 1024 codes eight), across teams of a wave and waves in f32 in a fixed order, across blocks and codes in f64.  At 129 x 1000
+// the loss is off by 1.4e-7 of it where f64 sums of f32 shares are by 0.9e-7.
+//
 // Scores are read once forward and once backward, which is the floor: 16384 x 8192 bf16, a fifth padded, 30 us at the 7.1 TB/s of loads alone and
-// 97 at the 4.97 TB/s of a copy.  Measured: rows 63 us, partial sums 12, loss 7; gradient 85 (non-temporal accesses: past the copy's rate).
-// Forward is bound by the one exchange over waves a row: 512 blocks of eight waves, two rows in flight; 256 blocks 89 us for the three kernels
-// where these take 80, 768 82, 1024 87 (more partial sums), four waves of four quads 78, sixteen of one 98.  16384 x 1024 f32: 21 + 5 + 4, gradient
-// 20.  Calls of some hundred rows are launches and the autograd engine: 18 us of kernels in 108 us, of which a step that does nothing takes 37.
+// 83 at the 5.84 TB/s of a copy.  Measured: rows 65 us, partial sums 12, loss 6; gradient 85 (non-temporal accesses: a copy's rate).
+// Forward: vector units busy 89 % of the time (12.5 instructions a score), an exchange over waves a row: 512 blocks of eight waves, two rows in
+// flight; 256 blocks 89 us for the three kernels where these take 80, 768 82, 1024 87 (more partial sums), four waves of four quads 78, sixteen of
+// one 98.  16384 x 1024 f32: 21 + 5 + 3, gradient 20.  Calls of some hundred rows are launches, the autograd engine and the wrapper: 18 us of
+// kernels in 105 us, of which a step that does nothing takes 37.
 #include "common.h"
 
 namespace mq {

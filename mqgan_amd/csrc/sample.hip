@@ -24,12 +24,13 @@
 // the bits of the score finds the cut instead.
 //
 // What bounds it: 16384 x 8192 f32 read once are 76 us at the 7.1 TB/s that loads alone reach here.  The maximum alone (temperature 0) takes 105
-// us, top-k 20 145, top-k 100 with top-p 0.95 200: two thirds of the latter is the issue of vector instructions, the rest waits of the lists'
-// waves.  Without top-k the masses of all codes are needed, 22 f64 operations each: 16384 x 8192 without a filter 280 us, top-p 0.95 530; 16384 x
-// 1024 with top-p 0.9 60 (floor 9.5), of which reading and the first masses are 32, the cut 20 and the draw 7.  Small calls are latency, a chain
-// of some thirty dependent LDS accesses and barriers: one row of 1000 codes with all filters 9 us, 48 of 8003 with top-p 0.95 25, 64 of 32000 with
-// top-k 100 and top-p 0.9 27.  Selection by the bits of the scores over a row in memory took 2688 us where the lists take 200; a row in registers
-// needs 215 of them.
+// us, top-k 20 145, top-k 100 with top-p 0.95 195-205: the vector units are busy 74 % of the latter (35 instructions a code), the rest is waits of the
+// lists' waves.  Without top-k the masses of all codes are needed, 15 sums, products and FMAs in f64 each beside scaling, rounding, conversion and
+// comparison: 16384 x 8192 without a filter 263-280 us (52 instructions a code, busy 76 %), top-p 0.95 530-590 (132, busy 90 %); 16384 x 1024 with
+// top-p 0.9 57-61 (floor 9.5; 99 a code, busy 85 %), of which reading and the first masses are 32, the cut 20 and the draw 7.  Small calls are latency,
+// a chain of some thirty dependent LDS accesses and barriers: one row of 1000 codes with all filters 10 us, 48 of 8003 with top-p 0.95 25, 64 of 32000
+// with top-k 100 and top-p 0.9 27.  Selection by the bits of the scores over a row in memory took 2688 us where the lists take 200; a row in
+// registers needs 215 of them.
 #include <algorithm>
 
 #include "common.h"
