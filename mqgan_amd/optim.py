@@ -42,9 +42,10 @@ class AdamW:
                 raise ValueError(f"AdamW: a group has params, weight_decay and lr_scale, not {sorted(unknown)}")
             mine = {}
             for p in g["params"]:
-                mine.setdefault(decays is None or bool(decays(p)), []).append(len(self.params))
+                decayed = decays is None or bool(decays(p))
+                mine.setdefault(decayed, []).append(len(self.params))
                 self.params.append(p)
-                self.weight_decays.append(float(g.get("weight_decay", weight_decay)) if decays is None or decays(p) else 0.0)
+                self.weight_decays.append(float(g.get("weight_decay", weight_decay)) if decayed else 0.0)
                 self.lr_scales.append(float(g.get("lr_scale", 1.0)))
             self.groups += [mine[k] for k in (True, False) if k in mine]
         if not self.params:
@@ -245,8 +246,9 @@ class AdamW:
 
     def load_state_dict(self, sd):
         """A state of this class or of torch.optim.AdamW (or Adam, train.FlatAdam).  Where its groups are this optimiser's - the same
-        tensors for a state of this class, the same numbers of them otherwise - lr, scales, weight decays, betas and eps come with it, as in
-        torch; where they are not, lr alone (the first group's) does and the tensors go by their position."""
+        tensors for a state of this class, the same numbers of them otherwise - lr, scales, betas and eps come with it, as in torch, and weight
+        decays where they are decoupled ones (Adam's is another thing); where they are not, lr alone (the first group's) does and the
+        tensors go by their position."""
         own = "mqgan_amd_calls" in sd
         saved = sd.get("param_groups") or []
         ids = [[int(i) for i in g["params"]] for g in saved]
@@ -308,6 +310,8 @@ class AdamW:
         self.weight_decays, self.lr_scales = list(before[0]), list(before[1])
         for group, g, scale in zip(self.groups, saved, scales):
             for i in group:
-                self.weight_decays[i], self.lr_scales[i] = float(g.get("weight_decay", before[0][i])), float(scale)
+                self.lr_scales[i] = float(scale)
+                if g.get("decoupled_weight_decay"):
+                    self.weight_decays[i] = float(g.get("weight_decay", before[0][i]))
         if (self.weight_decays, self.lr_scales) != before:
             self._bind(self._addresses)                 # both stand in the table

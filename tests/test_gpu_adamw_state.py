@@ -193,6 +193,29 @@ def test_states_of_other_groups_give_lr_and_moments_only():
     assert adam.lr == 7e-4 and adam.step_count == 4
 
 
+@pytest.mark.parametrize("kind", ["torch.optim.Adam", "FlatAdam"])
+def test_the_decay_of_adam_is_not_taken_for_a_decoupled_one(kind):
+    from mqgan_amd.ddp import FlatArena
+    from mqgan_amd.optim import AdamW
+    from mqgan_amd.train import FlatAdam
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.w = torch.nn.ParameterList(leaves())
+    if kind == "FlatAdam":
+        adam = FlatAdam(FlatArena([Net()]), 2e-3, (0.6, 0.8))
+        adam.step_count = 1
+    else:
+        qs = leaves()
+        adam = torch.optim.Adam(qs, lr=2e-3, betas=(0.6, 0.8), weight_decay=0.5)
+        give(qs, 0)
+        adam.step()
+    opt = AdamW(leaves(), lr=1.0, weight_decay=0.3)
+    opt.load_state_dict(adam.state_dict())
+    assert opt.weight_decays == [0.3] * 5 and (opt.lr, opt.betas) == (2e-3, (0.6, 0.8)) and opt._steps()[0] == [1] * 5
+
+
 def test_a_state_with_one_group_for_all_gives_lr_and_moments():
     """As this class wrote them at first: whatever the groups, one with the largest decay and the lr before scaling."""
     from mqgan_amd.optim import AdamW
